@@ -20,6 +20,12 @@ from dataclasses import dataclass
 
 import numpy as np
 
+from . import paged
+from .paged import (ELEM_BF16, ELEM_F16, ELEM_F32, SiPagedAppend, SiPagedAttention, SiPagedEvict, SiPagedKv,
+                    SiVerifyDrafts, paged_append, paged_attention, paged_attention_workspace_bytes, paged_evict,
+                    paged_evict_workspace_bytes, paged_kv, paged_kv_offset, rope_table, verify_drafts,
+                    verify_drafts_workspace_bytes)
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsi_cuda.so")
 
@@ -323,6 +329,7 @@ def lib():
         "si_ctx_comm_init": ([vp, i32, i32, vp], i32),
         "si_ctx_comm_info": ([vp, vp, vp], i32),
     }
+    sig.update(paged.SIGNATURES)
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
         fn.argtypes = args
@@ -802,6 +809,33 @@ class CudaContext:
         self._ck(lib().si_attention_layer_dev(self.h, C.byref(desc), _p(x), position, _p(key_cache),
                                               _p(value_cache), cached_tokens, capacity_tokens, _p(out), _p(work),
                                               stream))
+
+    # -- paged cache (include/si_paged.h; descriptions from paged.py) ---------
+    def _here(self, described):
+        """Refuses a description whose tensors are not on this context's GPU."""
+        held = getattr(described, "_tensors", None)
+        if held and (held[0].device.type != "cuda" or held[0].device.index != self.device):
+            raise SiError(SI_E_INVALID, f"tensors are on {held[0].device}, the context on cuda:{self.device}")
+
+    def paged_append_dev(self, kv: SiPagedKv, append: SiPagedAppend, stream=None):
+        """si_paged_append_dev: rotary positions of new queries and keys, keys and values into pages."""
+        self._here(kv)
+        self._ck(lib().si_paged_append_dev(self.h, C.byref(kv), C.byref(append), stream))
+
+    def paged_attention_dev(self, kv: SiPagedKv, attention: SiPagedAttention, stream=None):
+        """si_paged_attention_dev: attention of one new token a sequence over pages."""
+        self._here(kv)
+        self._ck(lib().si_paged_attention_dev(self.h, C.byref(kv), C.byref(attention), stream))
+
+    def paged_evict_dev(self, kv: SiPagedKv, evict: SiPagedEvict, stream=None):
+        """si_paged_evict_dev: every longer sequence cut to the budget by accumulated weight."""
+        self._here(kv)
+        self._ck(lib().si_paged_evict_dev(self.h, C.byref(kv), C.byref(evict), stream))
+
+    def verify_drafts_dev(self, drafts: SiVerifyDrafts, stream=None):
+        """si_verify_drafts_dev: drafted tokens against the target's probabilities."""
+        self._here(drafts)
+        self._ck(lib().si_verify_drafts_dev(self.h, C.byref(drafts), stream))
 
 
 class PeerBuffer:

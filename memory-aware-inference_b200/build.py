@@ -40,7 +40,7 @@ def _flags():
 
 def _deps():
     return glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + \
-        [os.path.join(REPO, "include", "si_cuda.h")]
+        glob.glob(os.path.join(REPO, "include", "*.h"))
 
 
 def _compile(src, force, verbose):

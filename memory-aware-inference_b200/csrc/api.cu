@@ -128,12 +128,13 @@ int sync_and_check(si_ctx* ctx, const char* what) {
   const int bits = *ctx->h_err;
   if (bits) {
     cudaMemset(ctx->d_err, 0, sizeof(int));
+    const bool gave_up = bits & (KERR_TIMEOUT_FULL | KERR_TIMEOUT_EMPTY | KERR_TIMEOUT_DRAIN);
     // a kernel that gave up may have left split-group counters behind
-    if (ctx->qscratch.p) cudaMemset(ctx->qscratch.p, 0, ctx->qscratch.cap);
+    if (gave_up && ctx->qscratch.p) cudaMemset(ctx->qscratch.p, 0, ctx->qscratch.cap);
     *ctx->h_err = 0;
-    return fail(ctx, bits & (KERR_TIMEOUT_FULL | KERR_TIMEOUT_EMPTY | KERR_TIMEOUT_DRAIN)
-                         ? SI_E_TIMEOUT
-                         : SI_E_CUDA,
+    if (!gave_up && bits == KERR_BAD_INDEX)  // a value that the caller passed in device memory
+      return fail(ctx, SI_E_INVALID, std::string(what) + ": a page, length, slot or token is out of range");
+    return fail(ctx, gave_up ? SI_E_TIMEOUT : SI_E_CUDA,
                 std::string(what) + ": device error bits " + std::to_string(bits));
   }
   return SI_OK;

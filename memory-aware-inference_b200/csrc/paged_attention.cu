@@ -1,0 +1,746 @@
+// Attention of one new token a sequence over a paged key-value cache.
+//
+// o = sum_t p_t v_t / sum_t p_t, p_t = exp(s_t - max s), s_t = scale q.k_t, for
+// the query heads that share a kv head. Every key and value is read once, so
+// the work is bound by HBM (2 flop a byte and query head) once a few thousand
+// tokens are in the batch, and by latency below that.
+//
+// Split. The unit of work is 16 consecutive slots of one (sequence, kv head,
+// block of 8 query heads). All units of the batch, in that order, are shared
+// out evenly over the warps of one resident CTA a multiprocessor, whatever the
+// lengths: the counts come from lengths on the device, so a call needs no host
+// copy of them and a captured call follows later lengths. A warp's share covers
+// the end of one (sequence, head), some whole ones, and the beginning of
+// another; whole ones are written at once, the partial ones (at most two a
+// warp) meet in shared memory after the CTA's only barrier, those that cross
+// the CTA's borders (at most two a CTA) in the workspace, which a second
+// kernel joins. Every join sums in a fixed order.
+//
+// A unit. Keys and values go from global memory straight into the registers
+// in which the tensor cores (mma.m16n8k16) want them; there is no shared-memory
+// stage and no barrier in the loop:
+//   S^T = K Q^T: the order of dims in the contraction is free as long as both
+//     operands share it, so a lane's 16-byte load of 8 dims of a key is the A
+//     operand of two steps. Lane (n, c) = (lane / 4, lane % 4) loads dims
+//     32 s + 8 c .. + 7 of slots n and n + 8.
+//   O^T = V^T P^T: the order of output rows (dims) is free too. The lane loads
+//     dims 64 d + 8 n .. + 7 of slots 2c, 2c + 1, 2c + 8, 2c + 9; byte
+//     permutes pair the slots, and output row r of step (d, j) is dim
+//     64 d + 8 n + 2j (+ 1 for rows 8..15), so a lane ends with 8 neighbouring
+//     dims of its two query heads.
+//   P leaves the first product transposed; movmatrix turns it into the second
+//     one's B operand.
+// The keys of the next unit are requested when this unit's scores are done,
+// its values after this unit's product, so loads are in flight throughout.
+//
+// Precision: queries are split into TQ 16-bit terms and probabilities into TP,
+// each multiplied separately into the same f32 accumulators. 16-bit queries of
+// the cache's own type are exact in one term. f32 queries take 3 bf16 terms
+// (24 bits) or 2 f16 terms (22 bits, after scaling each query by a power of two
+// to a maximum near 1), probabilities 3 bf16 or 2 f16 terms with f32 output and
+// 2 with 16-bit output. In f16, probabilities are scaled by 2^15 so that small ones keep
+// their bits; the sum is taken of the same scaled values.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "paged.cuh"
+
+namespace si {
+namespace {
+
+constexpr uint32_t kUnit = 16;  // slots of a unit
+constexpr uint32_t kCols = 8;   // query heads of a block
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <int HD>
+struct Shape {
+  static constexpr int kWarps = HD <= 128 ? 12 : 8;  // registers: 168 or 255 a thread
+  static constexpr int kK = HD / 32, kV = HD / 64;   // 16-byte loads a slot and lane
+};
+
+// Join records and partials in the workspace (one CTA: two partial slots).
+struct Join {
+  int32_t last;    // last CTA of the pair that crosses this CTA's first border; -1: none starts before it
+  uint32_t slot0;  // partial slot of the CTA before
+  uint32_t b, head;  // sequence; kv head * blocks + block
+};
+
+struct AttArgs {
+  PagedView kv;
+  const void* q;
+  void* out;
+  uint64_t q_ss, q_hs, o_ss, o_hs;
+  const int32_t* lengths;
+  float scale;  // times log2 e
+  uint32_t elem, qh, group, blocks;
+  bool q_wide, o_wide;
+  float* lse;      // natural log; may be null
+  float* lse2;     // log2, workspace of the weights pass; null without weights
+  float* scores;   // log2 scores [b * kvh + h][slot][gpad]; null without weights
+  uint32_t gpad;
+  float* part;     // [ctas][2][kCols][HD + 2]
+  Join* join;      // [ctas]
+  int* err;
+};
+
+__device__ __forceinline__ uint4 ldg_stream(const uint16_t* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma16(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Pair (x, y) rounded to 16 bits, and what the rounding left.
+template <bool BF16>
+__device__ __forceinline__ uint32_t take_term(float& x, float& y) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(x, y);
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&r);
+    x -= __uint_as_float(u << 16);
+    y -= __uint_as_float(u & 0xffff0000u);
+    return u;
+  } else {
+    const __half2 r = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(r);
+    x -= f.x;
+    y -= f.y;
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
+  return __shfl_sync(0xffffffffu, v, src);
+}
+
+// Where unit u lies. prefix[b] counts the 16-slot tiles of the sequences before b.
+struct Place {
+  uint32_t b, head, tile, tiles;
+};
+__device__ __forceinline__ Place place_of(uint64_t u, const uint32_t* prefix, uint32_t sequences, uint32_t heads) {
+  const uint64_t t = u / heads;  // tiles of earlier sequences all have `heads` units each
+  uint32_t lo = 0, hi = sequences;  // prefix[lo] <= t < prefix[hi]
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (prefix[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  Place p;
+  p.b = lo;
+  p.tiles = prefix[lo + 1] - prefix[lo];
+  const uint64_t in = u - uint64_t(prefix[lo]) * heads;
+  p.head = uint32_t(in / p.tiles);
+  p.tile = uint32_t(in - uint64_t(p.head) * p.tiles);
+  return p;
+}
+
+// prefix[0..sequences] of the tiles of every sequence, by the whole CTA.
+__device__ __forceinline__ void tile_prefix(const AttArgs& a, uint32_t* prefix, uint32_t* s_warp) {
+  const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  uint32_t run = 0;
+  if (threadIdx.x == 0) prefix[0] = 0;
+  for (uint32_t base = 0; base < a.kv.sequences; base += blockDim.x) {
+    const uint32_t i = base + threadIdx.x;
+    uint32_t n = 0;
+    if (i < a.kv.sequences) n = (checked_length(a.lengths[i], a.kv.max_tokens, a.err) + kUnit - 1) / kUnit;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= uint32_t(o)) n += v;
+    }
+    if (lane == 31) s_warp[w] = n;
+    __syncthreads();
+    uint32_t before = run;
+    for (uint32_t j = 0; j < nw; ++j) {
+      if (j < w) before += s_warp[j];
+      run += s_warp[j];
+    }
+    if (i < a.kv.sequences) prefix[i + 1] = before + n;
+    __syncthreads();
+  }
+}
+
+// First unit of share i of n. Units stay below 2^50 (2^32 tiles, 2^18 heads),
+// shares below 2^12.
+__device__ __forceinline__ uint64_t share(uint64_t units, uint32_t i, uint32_t n) { return units * i / n; }
+
+template <int HD, bool BF16, int TQ, int TP>
+__global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_kernel(const __grid_constant__ AttArgs a) {
+  constexpr int NW = Shape<HD>::kWarps, KK = Shape<HD>::kK, KV = Shape<HD>::kV;
+  constexpr float kShift = BF16 ? 0.f : 15.f;
+  constexpr uint32_t kPart = kCols * (HD + 2);                   // floats of a partial: values, then max and sum
+  constexpr uint32_t kQ = uint32_t(TQ * KK) * 32 * 4;            // floats of a warp's query terms
+  constexpr uint32_t kRegion = (kQ > kPart ? kQ : kPart) + kPart;
+  extern __shared__ __align__(16) float smem[];
+  // per warp: [query terms, later the partial of the last pair][partial of the first pair]
+  __shared__ uint32_t s_warp[NW];
+  __shared__ int64_t s_pair[NW][2];
+  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + NW * kRegion);
+  const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5, n8 = lane >> 2, c4 = lane & 3;
+  const uint32_t heads = a.kv.kv_heads * a.blocks;
+  if (threadIdx.x < 2 * NW) s_pair[threadIdx.x / 2][threadIdx.x % 2] = -1;
+  pdl_launch_dependents();
+  pdl_wait();
+  tile_prefix(a, prefix, s_warp);
+  const uint64_t units = uint64_t(prefix[a.kv.sequences]) * heads;
+  // rows of empty sequences
+  for (uint32_t b = blockIdx.x; b < a.kv.sequences; b += gridDim.x) {
+    if (prefix[b + 1] != prefix[b]) continue;
+    const float zero[8] = {};
+    for (uint32_t i = threadIdx.x; i < a.qh * (a.kv.hd / 8); i += NW * 32) {
+      const uint32_t h = i / (a.kv.hd / 8), ch = i - h * (a.kv.hd / 8);
+      store8(a.out, b * a.o_ss + h * a.o_hs + ch * 8, a.elem, a.o_wide, zero);
+    }
+    if (a.lse)
+      for (uint32_t h = threadIdx.x; h < a.qh; h += NW * 32) a.lse[uint64_t(b) * a.qh + h] = -INFINITY;
+  }
+  // few units: as many CTAs as give every warp one
+  const uint32_t ctas = uint32_t(min(uint64_t(gridDim.x), (units + NW - 1) / NW));
+  const uint32_t cta = blockIdx.x;
+  if (threadIdx.x == 0) {
+    Join j = {-1, 0, 0, 0};
+    if (cta > 0 && cta < ctas) {
+      const uint64_t cu = share(units, cta, ctas), before = share(units, cta - 1, ctas);
+      const Place p = place_of(cu, prefix, a.kv.sequences, heads);
+      const uint64_t first = cu - p.tile, end = first + p.tiles;
+      if (first < cu && first >= before) {  // the first border inside this pair
+        j.last = int32_t((end * ctas + units - 1) / units - 1);  // whose share holds unit end - 1
+        j.slot0 = first == before ? 0 : 1;
+        j.b = p.b;
+        j.head = p.head;
+      }
+    }
+    a.join[cta] = j;
+  }
+  if (cta >= ctas) return;
+  const uint64_t u0 = share(units, cta * NW + w, ctas * NW), u1 = share(units, cta * NW + w + 1, ctas * NW);
+  float* region = smem + w * kRegion;
+  uint4* s_q = reinterpret_cast<uint4*>(region) + lane;  // [term][step][lane]: a lane reads what it wrote
+  const uint32_t chunks = a.kv.hd / 8;
+
+  uint64_t u = u0;
+  while (u < u1) {
+    const Place at = place_of(u, prefix, a.kv.sequences, heads);
+    const uint32_t kvh = at.head / a.blocks, col0 = (at.head - kvh * a.blocks) * kCols;
+    const uint32_t cols = min(kCols, a.group - col0), qhead0 = kvh * a.group + col0;
+    const uint32_t t_end = uint32_t(min(uint64_t(at.tiles), at.tile + (u1 - u)));
+    const uint32_t len = checked_length(a.lengths[at.b], a.kv.max_tokens, a.err);
+    const int32_t* row = a.kv.pages + at.b * a.kv.pages_stride;
+
+    // queries into 16-bit terms; columns past the group are zero
+    float col_scale = a.scale;
+    {
+      float q[KK][8];
+      float big = 0.f;
+#pragma unroll
+      for (int s = 0; s < KK; ++s) {
+        const uint32_t ch = 4 * s + c4;
+        if (n8 < cols && ch < chunks) {
+          load8(a.q, at.b * a.q_ss + (qhead0 + n8) * a.q_hs + ch * 8, a.elem, a.q_wide, q[s]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) q[s][j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(q[s][j]));
+      }
+      if constexpr (!BF16) {  // to a maximum in [1, 2): f16 has no exponent to spare
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        int e = 0;
+        if (big > 0.f && big < INFINITY) e = max(-100, ilogbf(big));
+        const float down = ldexpf(1.f, -e);
+        col_scale *= ldexpf(1.f, e);
+#pragma unroll
+        for (int s = 0; s < KK; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) q[s][j] *= down;
+      }
+#pragma unroll
+      for (int s = 0; s < KK; ++s)
+#pragma unroll
+        for (int t = 0; t < TQ; ++t) {
+          uint4 r;
+          r.x = take_term<BF16>(q[s][0], q[s][1]);
+          r.y = take_term<BF16>(q[s][2], q[s][3]);
+          r.z = take_term<BF16>(q[s][4], q[s][5]);
+          r.w = take_term<BF16>(q[s][6], q[s][7]);
+          s_q[(t * KK + s) * 32] = r;
+        }
+    }
+    // scale of the lane's two columns of S^T
+    const float sc0 = __shfl_sync(0xffffffffu, col_scale, c4 * 8), sc1 = __shfl_sync(0xffffffffu, col_scale, c4 * 8 + 4);
+
+    float acc[KV * 4][4] = {};
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    uint4 kr[2][KK], vr[4][KV];
+
+    // The page of slot (unit, lane % 16), asked for two units ahead of its use;
+    // a negative number stands for "no slot".
+    auto page_of = [&](uint32_t tile) -> int32_t {
+      const uint32_t t = tile * kUnit + (lane & 15);
+      return tile < t_end && t < len ? __ldg(row + div_of(t, a.kv.page)) : -1;
+    };
+    auto cell_of = [&](uint32_t tile, int32_t page) -> uint64_t {
+      const uint32_t t = tile * kUnit + (lane & 15);
+      const uint64_t cell = paged_cell(a.kv, page, t - div_of(t, a.kv.page) * a.kv.page.d, kvh);
+      if (cell == kNoCell && tile < t_end && t < len) atomicOr(a.err, KERR_BAD_INDEX);
+      return cell;
+    };
+    auto load_k = [&](uint64_t cell, bool& lo, bool& hi) {
+      const uint64_t c0 = shfl64(cell, n8), c1 = shfl64(cell, n8 + 8);
+      lo = c0 != kNoCell;
+      hi = c1 != kNoCell;
+#pragma unroll
+      for (int s = 0; s < KK; ++s) {
+        const uint32_t ch = 4 * s + c4;
+        kr[0][s] = lo && ch < chunks ? ldg_stream(a.kv.k + c0 + ch * 8) : make_uint4(0, 0, 0, 0);
+        kr[1][s] = hi && ch < chunks ? ldg_stream(a.kv.k + c1 + ch * 8) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto load_v = [&](uint64_t cell) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t c = shfl64(cell, 2 * c4 + (i & 1) + (i >> 1) * 8);
+#pragma unroll
+        for (int d = 0; d < KV; ++d) {
+          const uint32_t ch = 8 * d + n8;
+          vr[i][d] = c != kNoCell && ch < chunks ? ldg_stream(a.kv.v + c + ch * 8) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    };
+
+    bool lo, hi;
+    uint64_t cell = cell_of(at.tile, page_of(at.tile));
+    int32_t page_next = page_of(at.tile + 1);
+    load_k(cell, lo, hi);
+    load_v(cell);
+    for (uint32_t tile = at.tile; tile < t_end; ++tile) {
+      const int32_t page_after = page_of(tile + 2);
+      float s[4] = {};
+#pragma unroll
+      for (int st = 0; st < KK; ++st) {
+        const uint4 x = kr[0][st], y = kr[1][st];
+        const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+        for (int t = TQ - 1; t >= 0; --t) {  // small terms first
+          const uint4 qv = s_q[(t * KK + st) * 32];
+          mma16<BF16>(s, a0, qv.x, qv.y);
+          mma16<BF16>(s, a1, qv.z, qv.w);
+        }
+      }
+      const bool lo_now = lo, hi_now = hi;
+      cell = cell_of(tile + 1, page_next);
+      page_next = page_after;
+      load_k(cell, lo, hi);
+      // base-2 scores; slots that do not exist leave nothing
+      s[0] = lo_now ? s[0] * sc0 : -INFINITY;
+      s[1] = lo_now ? s[1] * sc1 : -INFINITY;
+      s[2] = hi_now ? s[2] * sc0 : -INFINITY;
+      s[3] = hi_now ? s[3] * sc1 : -INFINITY;
+      if (a.scores) {
+        float* to = a.scores + (uint64_t(at.b * a.kv.kv_heads + kvh) * a.kv.max_tokens + tile * kUnit) * a.gpad + col0 + 2 * c4;
+        if (2 * c4 < cols) {  // gpad is even: the pair's second place exists
+          if (tile * kUnit + n8 < len) *reinterpret_cast<float2*>(to + uint64_t(n8) * a.gpad) = make_float2(s[0], s[1]);
+          if (tile * kUnit + n8 + 8 < len)
+            *reinterpret_cast<float2*>(to + uint64_t(n8 + 8) * a.gpad) = make_float2(s[2], s[3]);
+        }
+      }
+      float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
+      }
+      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {  // the running maximum moves seldom after the first units
+        const float g0 = fmaxf(m0, x0), g1 = fmaxf(m1, x1);
+        const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - g0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - g1);
+        m0 = g0;
+        m1 = g1;
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int i = 0; i < KV * 4; ++i) {
+          acc[i][0] *= f0;
+          acc[i][1] *= f1;
+          acc[i][2] *= f0;
+          acc[i][3] *= f1;
+        }
+      }
+      const float b0 = m0 == -INFINITY ? 0.f : m0 - kShift, b1 = m1 == -INFINITY ? 0.f : m1 - kShift;
+      float p[4] = {exp2f(s[0] - b0), exp2f(s[1] - b1), exp2f(s[2] - b0), exp2f(s[3] - b1)};
+      l0 += p[0] + p[2];
+      l1 += p[1] + p[3];
+      uint32_t pb[TP][2];
+#pragma unroll
+      for (int t = 0; t < TP; ++t) {
+        pb[t][0] = transpose8(take_term<BF16>(p[0], p[1]));
+        pb[t][1] = transpose8(take_term<BF16>(p[2], p[3]));
+      }
+#pragma unroll
+      for (int d = 0; d < KV; ++d) {
+        const uint32_t v0[4] = {vr[0][d].x, vr[0][d].y, vr[0][d].z, vr[0][d].w};
+        const uint32_t v1[4] = {vr[1][d].x, vr[1][d].y, vr[1][d].z, vr[1][d].w};
+        const uint32_t v2[4] = {vr[2][d].x, vr[2][d].y, vr[2][d].z, vr[2][d].w};
+        const uint32_t v3[4] = {vr[3][d].x, vr[3][d].y, vr[3][d].z, vr[3][d].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t av[4] = {__byte_perm(v0[j], v1[j], 0x5410), __byte_perm(v0[j], v1[j], 0x7632),
+                                  __byte_perm(v2[j], v3[j], 0x5410), __byte_perm(v2[j], v3[j], 0x7632)};
+#pragma unroll
+          for (int t = TP - 1; t >= 0; --t) mma16<BF16>(acc[d * 4 + j], av, pb[t][0], pb[t][1]);
+        }
+      }
+      load_v(cell);
+    }
+    // sums of the lane's two columns over the slots
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+    }
+    if (at.tile == 0 && t_end == at.tiles) {  // a whole pair
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t col = 2 * c4 + c;
+        if (col >= cols) continue;
+        const float l = c ? l1 : l0, inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int d = 0; d < KV; ++d) {
+          const uint32_t ch = 8 * d + n8;
+          if (ch >= chunks) continue;
+          float o[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            o[2 * j] = acc[d * 4 + j][c] * inv;
+            o[2 * j + 1] = acc[d * 4 + j][2 + c] * inv;
+          }
+          store8(a.out, at.b * a.o_ss + (qhead0 + col) * a.o_hs + ch * 8, a.elem, a.o_wide, o);
+        }
+        if (n8 == 0) {
+          const float z = l > 0.f ? (c ? m1 : m0) - kShift + log2f(l) : -INFINITY;
+          const uint64_t i = uint64_t(at.b) * a.qh + qhead0 + col;
+          if (a.lse) a.lse[i] = z * kLn2;
+          if (a.lse2) a.lse2[i] = z;
+        }
+      }
+    } else {
+      // the share's first pair beside the queries, another one over them
+      const uint32_t slot = u == u0 ? 0 : 1;
+      float* part = slot ? region : region + (kRegion - kPart);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t col = 2 * c4 + c;
+#pragma unroll
+        for (int d = 0; d < KV; ++d) {
+          float* to = part + col * HD + (8 * d + n8) * 8;
+          *reinterpret_cast<float4*>(to) =
+              make_float4(acc[d * 4][c], acc[d * 4][2 + c], acc[d * 4 + 1][c], acc[d * 4 + 1][2 + c]);
+          *reinterpret_cast<float4*>(to + 4) =
+              make_float4(acc[d * 4 + 2][c], acc[d * 4 + 2][2 + c], acc[d * 4 + 3][c], acc[d * 4 + 3][2 + c]);
+        }
+        if (n8 == 0) {
+          part[kCols * HD + 2 * col] = c ? m1 : m0;
+          part[kCols * HD + 2 * col + 1] = c ? l1 : l0;
+        }
+      }
+      if (lane == 0) s_pair[w][slot] = int64_t(u - at.tile);  // the pair's first unit names it
+    }
+    u += t_end - at.tile;
+  }
+  __syncthreads();
+  // join the warps' partials, in the order of their units
+  const uint64_t cu0 = share(units, cta, ctas), cu1 = share(units, cta + 1, ctas);
+  for (uint32_t e = 0; e < 2 * NW;) {
+    const int64_t pair = s_pair[e / 2][e % 2];
+    if (pair < 0) {
+      ++e;
+      continue;
+    }
+    uint32_t stop = e + 1;
+    while (stop < 2 * NW && (s_pair[stop / 2][stop % 2] < 0 || s_pair[stop / 2][stop % 2] == pair)) ++stop;
+    const Place at = place_of(uint64_t(pair), prefix, a.kv.sequences, heads);
+    const uint32_t kvh = at.head / a.blocks, col0 = (at.head - kvh * a.blocks) * kCols;
+    const uint32_t cols = min(kCols, a.group - col0), qhead0 = kvh * a.group + col0;
+    const bool whole = uint64_t(pair) >= cu0 && uint64_t(pair) + at.tiles <= cu1;
+    float* part = a.part + (uint64_t(cta) * 2 + (uint64_t(pair) <= cu0 ? 0 : 1)) * kPart;
+    for (uint32_t i = threadIdx.x; i < cols * (HD / 8); i += NW * 32) {
+      const uint32_t col = i / (HD / 8), ch = i - col * (HD / 8);
+      float m = -INFINITY;
+      for (uint32_t x = e; x < stop; ++x)
+        if (s_pair[x / 2][x % 2] >= 0)
+          m = fmaxf(m, (smem + (x / 2) * kRegion + (x % 2 ? 0 : kRegion - kPart))[kCols * HD + 2 * col]);
+      float l = 0.f, o[8] = {};
+      for (uint32_t x = e; x < stop; ++x) {
+        if (s_pair[x / 2][x % 2] < 0) continue;
+        const float* from = smem + (x / 2) * kRegion + (x % 2 ? 0 : kRegion - kPart);
+        const float mx = from[kCols * HD + 2 * col];
+        if (mx == -INFINITY) continue;
+        const float f = exp2f(mx - m);
+        l += f * from[kCols * HD + 2 * col + 1];
+        const float4 v0 = *reinterpret_cast<const float4*>(from + col * HD + ch * 8);
+        const float4 v1 = *reinterpret_cast<const float4*>(from + col * HD + ch * 8 + 4);
+        o[0] += f * v0.x, o[1] += f * v0.y, o[2] += f * v0.z, o[3] += f * v0.w;
+        o[4] += f * v1.x, o[5] += f * v1.y, o[6] += f * v1.z, o[7] += f * v1.w;
+      }
+      if (whole) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] *= inv;
+        if (ch < chunks) store8(a.out, at.b * a.o_ss + (qhead0 + col) * a.o_hs + ch * 8, a.elem, a.o_wide, o);
+        if (ch == 0) {
+          const float z = l > 0.f ? m - kShift + log2f(l) : -INFINITY;
+          const uint64_t y = uint64_t(at.b) * a.qh + qhead0 + col;
+          if (a.lse) a.lse[y] = z * kLn2;
+          if (a.lse2) a.lse2[y] = z;
+        }
+      } else {
+        *reinterpret_cast<float4*>(part + col * HD + ch * 8) = make_float4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<float4*>(part + col * HD + ch * 8 + 4) = make_float4(o[4], o[5], o[6], o[7]);
+        if (ch == 0) {
+          part[kCols * HD + 2 * col] = m;
+          part[kCols * HD + 2 * col + 1] = l;
+        }
+      }
+    }
+    e = stop;
+  }
+}
+
+// Joins the partials of the pairs that cross CTA borders. Block (i, column):
+// the pair whose first border is the one before CTA i, one query head of it.
+template <int HD>
+__global__ void __launch_bounds__(HD) paged_join_kernel(const __grid_constant__ AttArgs a, float shift) {
+  constexpr uint32_t kPart = kCols * (HD + 2);
+  pdl_launch_dependents();
+  pdl_wait();
+  const Join j = a.join[blockIdx.x + 1];
+  if (j.last < 0) return;
+  const uint32_t kvh = j.head / a.blocks, col0 = (j.head - kvh * a.blocks) * kCols, col = blockIdx.y;
+  if (col >= min(kCols, a.group - col0)) return;
+  const uint32_t first = blockIdx.x, d = threadIdx.x;  // CTA before the border
+  auto part = [&](uint32_t c) { return a.part + (uint64_t(c) * 2 + (c == first ? j.slot0 : 0)) * kPart; };
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  for (uint32_t c = first; c <= uint32_t(j.last); c += 8) {
+    float mx[8], lx[8], vx[8];
+    float g = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool in = c + i <= uint32_t(j.last);
+      const float* p = part(in ? c + i : first);
+      mx[i] = in ? p[kCols * HD + 2 * col] : -INFINITY;
+      lx[i] = p[kCols * HD + 2 * col + 1];
+      vx[i] = p[col * HD + d];
+      g = fmaxf(g, mx[i]);
+    }
+    if (g == -INFINITY) continue;
+    const float f = exp2f(m - g);
+    l *= f;
+    o *= f;
+    m = g;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = mx[i] == -INFINITY ? 0.f : exp2f(mx[i] - g);
+      l += f * lx[i];
+      o += f * vx[i];
+    }
+  }
+  const uint32_t head = kvh * a.group + col0 + col;
+  if (d < a.kv.hd) {
+    const uint64_t at = j.b * a.o_ss + head * a.o_hs + d;
+    const float v = l > 0.f ? o / l : 0.f;
+    if (a.elem == SI_ELEM_F32) static_cast<float*>(a.out)[at] = v;
+    else static_cast<uint16_t*>(a.out)[at] = f_to_elem(v, a.elem);
+  }
+  if (d == 0) {
+    const float z = l > 0.f ? m - shift + log2f(l) : -INFINITY;
+    const uint64_t y = uint64_t(j.b) * a.qh + head;
+    if (a.lse) a.lse[y] = z * kLn2;
+    if (a.lse2) a.lse2[y] = z;
+  }
+}
+
+// weights_out = weights_in + the group's probabilities, from the stored scores.
+__global__ void __launch_bounds__(256) paged_weights_kernel(const __grid_constant__ AttArgs a, const float* w_in,
+                                                            float* w_out, uint64_t stride) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t row = blockIdx.y, b = row / a.kv.kv_heads, h = row - b * a.kv.kv_heads;
+  const uint32_t len = checked_length(a.lengths[b], uint32_t(min(uint64_t(a.kv.max_tokens), stride)), a.err);
+  const float* z = a.lse2 + uint64_t(b) * a.qh + h * a.group;
+  for (uint32_t t = blockIdx.x * 256 + threadIdx.x; t < len; t += gridDim.x * 256) {
+    const float* s = a.scores + (uint64_t(row) * a.kv.max_tokens + t) * a.gpad;
+    float sum = 0.f;
+    for (uint32_t g = 0; g < a.group; g += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(s + g);
+      // a score of -inf is a slot that was left out: it has no weight
+      sum += x.x == -INFINITY ? 0.f : exp2f(x.x - z[g]);
+      if (g + 1 < a.group) sum += x.y == -INFINITY ? 0.f : exp2f(x.y - z[g + 1]);
+    }
+    const uint64_t i = uint64_t(row) * stride + t;
+    w_out[i] = (w_in ? w_in[i] : 0.f) + sum;
+  }
+}
+
+uint32_t padded_dim(uint32_t hd) { return (hd + 63) / 64 * 64; }
+uint32_t warps_of(uint32_t hd) { return padded_dim(hd) <= 128 ? 12 : 8; }
+
+// Workspace: join records, partials, then lse and scores of the weights pass.
+// The grid is one CTA a multiprocessor, so kMaxCtas bounds both.
+constexpr uint32_t kMaxCtas = 256;
+uint64_t part_bytes(uint32_t hd) { return uint64_t(kMaxCtas) * 2 * kCols * (padded_dim(hd) + 2) * 4; }
+uint64_t round16(uint64_t n) { return (n + 15) & ~uint64_t(15); }
+uint64_t work_bytes(const si_paged_kv& kv, uint32_t qh, bool weights) {
+  uint64_t n = kMaxCtas * sizeof(Join) + part_bytes(kv.head_dim);
+  if (weights) {
+    const uint32_t group = qh / kv.kv_heads, gpad = (group + 1) & ~1u;
+    n += round16(uint64_t(kv.sequences) * qh * 4);
+    n += uint64_t(kv.sequences) * kv.kv_heads * kv.max_pages * kv.page_tokens * gpad * 4;
+  }
+  return n;
+}
+
+int check_heads(const si_paged_kv* kv, uint32_t qh, std::string* msg) {
+  if (int rc = check_paged_kv(kv, msg)) return rc;
+  if (qh == 0 || qh % kv->kv_heads || qh > 65535) {
+    *msg = "paged attention query heads must be a multiple of the kv heads";
+    return SI_E_INVALID;
+  }
+  return SI_OK;
+}
+
+int check_attention(const si_paged_kv* kv, const si_paged_attention* a, std::string* msg) {
+  auto bad = [&](int rc, const std::string& text) {
+    *msg = text;
+    return rc;
+  };
+  if (!a) return bad(SI_E_INVALID, "null paged attention description");
+  if (int rc = check_heads(kv, a->query_heads, msg)) return rc;
+  if (!elem_known(a->elem)) return bad(SI_E_UNSUPPORTED, "paged attention elements must be f32, bf16 or f16");
+  if (!a->q || !a->out || !a->lengths) return bad(SI_E_INVALID, "paged attention buffers are null");
+  if (!elem_aligned(a->q, a->elem) || !elem_aligned(a->out, a->elem))
+    return bad(SI_E_INVALID, "paged attention buffers are not aligned to their elements");
+  if (!(a->scale >= 0.f) || a->scale > 3e38f) return bad(SI_E_INVALID, "paged attention scale must be finite and not negative");
+  if (a->weights_in && !a->weights_out) return bad(SI_E_INVALID, "paged attention has weights in and none out");
+  for (uint64_t s : {a->q_seq_stride, a->q_head_stride, a->out_seq_stride, a->out_head_stride, a->weights_stride})
+    if (s >> 44) return bad(SI_E_INVALID, "paged attention strides are out of range");
+  if (a->weights_out && a->weights_stride == 0) return bad(SI_E_INVALID, "paged attention weights have no stride");
+  if (a->weights_out && uint64_t(kv->sequences) * kv->kv_heads > 65535)
+    return bad(SI_E_UNSUPPORTED, "paged attention weights take at most 65535 sequences times kv heads");
+  const uint64_t need = work_bytes(*kv, a->query_heads, a->weights_out != nullptr);
+  if (!a->work || reinterpret_cast<uintptr_t>(a->work) % 16 || a->work_bytes < need)
+    return bad(SI_E_INVALID, "paged attention needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
+  return SI_OK;
+}
+
+template <int HD, bool BF16, int TQ, int TP>
+cudaError_t launch(const AttArgs& p, uint32_t grid, cudaStream_t s) {
+  constexpr uint32_t kPart = kCols * (HD + 2), kQ = uint32_t(TQ * (HD / 32)) * 32 * 4;
+  constexpr uint32_t kRegion = (kQ > kPart ? kQ : kPart) + kPart;
+  const uint32_t smem = Shape<HD>::kWarps * kRegion * 4 + (p.kv.sequences + 1) * 4;
+  static std::atomic<uint32_t> cache[kMaxDevices];
+  auto kernel = paged_attention_kernel<HD, BF16, TQ, TP>;
+  if (cudaError_t e = raise_smem_limit(kernel, smem, cache)) return e;
+  PdlLaunch l(dim3(grid), dim3(Shape<HD>::kWarps * 32), smem, s);
+  if (cudaError_t e = cudaLaunchKernelEx(&l.cfg, kernel, p)) return e;
+  if (grid == 1) return cudaSuccess;
+  PdlLaunch j(dim3(grid - 1, std::min(kCols, p.group)), dim3(HD), 0, s);
+  return cudaLaunchKernelEx(&j.cfg, paged_join_kernel<HD>, p, BF16 ? 0.f : 15.f);
+}
+
+template <int HD>
+cudaError_t launch_hd(const AttArgs& p, bool bf16, uint32_t grid, cudaStream_t s) {
+  if (bf16) {
+    if (p.elem == SI_ELEM_BF16) return launch<HD, true, 1, 2>(p, grid, s);
+    return launch<HD, true, 3, 3>(p, grid, s);
+  }
+  if (p.elem == SI_ELEM_F16) return launch<HD, false, 1, 2>(p, grid, s);
+  return launch<HD, false, 2, 2>(p, grid, s);
+}
+
+}  // namespace
+}  // namespace si
+
+using namespace si;
+
+extern "C" int si_paged_attention_workspace(const si_paged_kv* kv, uint32_t query_heads, int weights, uint64_t* bytes) {
+  std::string msg;
+  if (int rc = check_heads(kv, query_heads, &msg)) return fail(nullptr, rc, msg);
+  if (!bytes) return fail(nullptr, SI_E_INVALID, "null workspace size");
+  *bytes = work_bytes(*kv, query_heads, weights != 0);
+  return SI_OK;
+}
+
+extern "C" int si_paged_attention_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_attention* a, void* stream) {
+  std::string msg;
+  if (int rc = check_attention(kv, a, &msg)) return fail(ctx, rc, msg);
+  if (!ctx) return fail(nullptr, SI_E_INVALID, "null context");
+  DeviceGuard dev(ctx->device);
+  if (dev.e != cudaSuccess) return cuda_fail(ctx, dev.e, "paged attention device");
+  AttArgs p = {};
+  p.kv = paged_view(*kv);
+  p.q = a->q, p.out = a->out;
+  p.q_ss = a->q_seq_stride, p.q_hs = a->q_head_stride, p.o_ss = a->out_seq_stride, p.o_hs = a->out_head_stride;
+  p.lengths = a->lengths;
+  p.scale = (a->scale > 0.f ? a->scale : 1.f / std::sqrt(float(kv->head_dim))) * kLog2e;
+  p.elem = a->elem;
+  p.qh = a->query_heads;
+  p.group = a->query_heads / kv->kv_heads;
+  p.blocks = (p.group + kCols - 1) / kCols;
+  p.q_wide = wide_ok(a->q, a->elem, p.q_ss, p.q_hs);
+  p.o_wide = wide_ok(a->out, a->elem, p.o_ss, p.o_hs);
+  p.lse = a->lse;
+  p.gpad = (p.group + 1) & ~1u;
+  p.err = ctx->d_err;
+  uint8_t* work = static_cast<uint8_t*>(a->work);
+  p.join = reinterpret_cast<Join*>(work);
+  p.part = reinterpret_cast<float*>(work + kMaxCtas * sizeof(Join));
+  if (a->weights_out) {
+    uint8_t* more = work + kMaxCtas * sizeof(Join) + part_bytes(kv->head_dim);
+    p.lse2 = reinterpret_cast<float*>(more);
+    p.scores = reinterpret_cast<float*>(more + round16(uint64_t(kv->sequences) * p.qh * 4));
+  }
+  const cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
+  const uint64_t most = uint64_t(kv->sequences) * ((p.kv.max_tokens + kUnit - 1) / kUnit) * kv->kv_heads * p.blocks;
+  const uint32_t nw = warps_of(kv->head_dim);
+  const uint32_t grid = uint32_t(std::min<uint64_t>(std::min<uint32_t>(ctx->sm_count, kMaxCtas), (most + nw - 1) / nw));
+  const bool bf16 = kv->elem == SI_ELEM_BF16;
+  cudaError_t e;
+  switch (padded_dim(kv->head_dim)) {
+    case 64: e = launch_hd<64>(p, bf16, grid, s); break;
+    case 128: e = launch_hd<128>(p, bf16, grid, s); break;
+    case 192: e = launch_hd<192>(p, bf16, grid, s); break;
+    default: e = launch_hd<256>(p, bf16, grid, s); break;
+  }
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "paged attention launch");
+  if (a->weights_out) {
+    const uint32_t rows = kv->sequences * kv->kv_heads;
+    const uint32_t blocks = std::min<uint32_t>((p.kv.max_tokens + 255) / 256, std::max(1u, uint32_t(ctx->sm_count) * 8 / rows));
+    PdlLaunch l(dim3(blocks, rows), dim3(256), 0, s);
+    e = cudaLaunchKernelEx(&l.cfg, paged_weights_kernel, p, a->weights_in, a->weights_out, a->weights_stride);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "paged attention weights launch");
+  }
+  note_async_submission(ctx);
+  return SI_OK;
+}

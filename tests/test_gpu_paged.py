@@ -1,0 +1,801 @@
+"""Paged-cache operators on the GPU against plain 64-bit implementations.
+
+Tolerances. f32 outputs: the parity bound of this library's f32 operators, 1e-5
+relative L2. 16-bit outputs: the rounding of each value, at most half a step
+(eps / 2 relative), on top of that. Moves, counts and tokens are exact."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import load_package
+
+pytestmark = pytest.mark.gpu
+mai = load_package()
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+LEGACY = 1  # handle of torch's default stream
+
+
+def half_step(t):
+    return 0.0 if t == F32 else torch.finfo(t).eps / 2
+
+
+def close(got, want, dtype, f32_bound=1e-5):
+    got, want = got.double().cpu(), want.double().cpu()
+    assert torch.isfinite(got).all()
+    norm = want.norm()
+    assert (got - want).norm() <= (f32_bound + half_step(dtype)) * norm, ((got - want).norm() / norm).item()
+
+
+class Cache:
+    """Pools in any order of pages, heads and tokens; what no slot in use needs holds NaN."""
+
+    def __init__(self, lengths, kv_heads, page, hd, dtype=BF16, order="heads_first", spare=2, cols=None, seed=0, room=0):
+        gen = torch.Generator().manual_seed(seed)
+        need = [-(-max(n, 0) // page) + (room if n >= 0 else 0) for n in lengths]
+        self.cols = cols or max(1, max(need))
+        total = sum(need) + spare
+        shape = (total, kv_heads, page, hd) if order == "heads_first" else (total, page, kv_heads, hd)
+        self.k = torch.full(shape, math.nan, dtype=dtype, device="cuda")
+        self.v = torch.full(shape, math.nan, dtype=dtype, device="cuda")
+        if order != "heads_first":
+            self.k, self.v = self.k.transpose(1, 2), self.v.transpose(1, 2)
+        ids = torch.randperm(total, generator=gen)[:sum(need)].tolist()
+        self.pages = torch.full((len(lengths), self.cols), -7, dtype=torch.int32)
+        for b, n in enumerate(need):
+            for j in range(n):
+                self.pages[b, j] = ids.pop()
+        self.lengths = list(lengths)
+        self.page = page
+        for b, n in enumerate(lengths):
+            if n > 0:
+                pg, at = self.cells(b, n)
+                self.k[pg, :, at] = torch.randn(n, kv_heads, hd, generator=gen).to(dtype).cuda()
+                self.v[pg, :, at] = torch.randn(n, kv_heads, hd, generator=gen).to(dtype).cuda()
+        self.pages_dev = self.pages.cuda()
+        self.len_dev = torch.tensor(self.lengths, dtype=torch.int32, device="cuda")
+        self.desc = mai.paged_kv(self.k, self.v, self.pages_dev)
+
+    def cells(self, b, n):
+        t = torch.arange(n)
+        return self.pages[b].long()[t // self.page].cuda(), (t % self.page).cuda()
+
+    def rows(self, b, n, pool):
+        pg, at = self.cells(b, n)
+        return pool[pg, :, at].double()  # [n][kv_heads][hd]
+
+
+def reference(cache, q, scale=None, lengths=None):
+    """Attention, log-sum-exp and the group's probabilities in 64 bits."""
+    b_n, qh, hd = q.shape
+    kvh = cache.k.shape[1]
+    g = qh // kvh
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    lse = torch.full((b_n, qh), -math.inf, dtype=torch.float64, device="cuda")
+    weights = []
+    for b, n in enumerate(lengths or cache.lengths):
+        if n <= 0:
+            weights.append(None)
+            continue
+        k, v = cache.rows(b, n, cache.k), cache.rows(b, n, cache.v)
+        s = torch.einsum("hgd,nhd->hgn", q[b].double().view(kvh, g, hd), k) * (scale or hd ** -0.5)
+        p = torch.softmax(s, -1)
+        out[b] = torch.einsum("hgn,nhd->hgd", p, v).reshape(qh, hd)
+        lse[b] = torch.logsumexp(s, -1).view(-1)
+        weights.append(p.sum(1))
+    return out, lse, weights
+
+
+def work_for(cache, qh, weights=False):
+    return torch.empty(mai.paged_attention_workspace_bytes(cache.desc, qh, weights), dtype=torch.uint8, device="cuda")
+
+
+def attend(ctx, cache, q, out=None, stream=LEGACY, **kw):
+    out = torch.full_like(q, math.nan) if out is None else out
+    work = work_for(cache, q.shape[1], kw.get("weights_out") is not None).fill_(255)
+    args = mai.paged_attention(cache.desc, q, out, cache.len_dev, work, **kw)
+    ctx.paged_attention_dev(cache.desc, args, stream)
+    return out
+
+
+ATTENTION = [
+    # lengths, kv_heads, group, head_dim, page
+    ([1], 1, 1, 64, 1),
+    ([0], 1, 1, 64, 16),
+    ([15, 16, 17, 0, 31, 32, 33], 2, 1, 64, 16),
+    ([1, 2, 3, 0, 5], 4, 6, 256, 16),
+    ([517], 4, 6, 256, 16),
+    ([100, 0, 0, 7], 1, 8, 128, 5),
+    ([129, 63, 1], 2, 3, 80, 24),
+    ([300, 299], 5, 12, 96, 7),
+    ([64], 1, 17, 192, 64),
+    ([1000] * 3, 2, 2, 8, 32),
+    ([777, 12], 3, 5, 40, 1),
+    ([4096, 1, 2048], 2, 4, 128, 256),
+    ([20000], 1, 7, 256, 48),
+    (list(range(0, 400, 3)), 2, 4, 128, 16),
+    ([40] * 700, 1, 1, 64, 16),
+]
+
+
+@pytest.mark.parametrize("io, cache_type", [(F32, BF16), (BF16, BF16), (F32, F16), (F16, F16), (BF16, F16), (F16, BF16)])
+@pytest.mark.parametrize("case", range(len(ATTENTION)))
+def test_attention(ctx, case, io, cache_type):
+    lengths, kvh, g, hd, page = ATTENTION[case]
+    cache = Cache(lengths, kvh, page, hd, cache_type, order="heads_first" if case % 2 else "tokens_first", seed=case)
+    q = torch.randn(len(lengths), kvh * g, hd, device="cuda").to(io)
+    lse = torch.full((len(lengths), kvh * g), math.nan, device="cuda")
+    out = attend(ctx, cache, q, lse=lse)
+    want, want_lse, _ = reference(cache, q)
+    ctx.synchronize()
+    close(out, want, io)
+    empty = want_lse == -math.inf
+    assert (lse[empty] == -math.inf).all() and (out[empty] == 0).all()
+    if not empty.all():
+        # log-sum-exp: absolute, as scores of size |q||k| round; 2^-16 covers 256 products of size 16 at 2^-24
+        assert (lse.double() - want_lse)[~empty].abs().max() <= 2 ** -16
+
+
+@pytest.mark.parametrize("scale", [0.0, 0.02, 1.7])
+@pytest.mark.parametrize("size", [1e-4, 1.0, 300.0])
+def test_attention_scales_and_ranges(ctx, scale, size):
+    """Small and large queries (one-hot softmax at 300), and f16 values that bf16 terms could not hold."""
+    for dtype in (BF16, F16):
+        cache = Cache([333, 48], 2, 16, 128, dtype, seed=3)
+        q = torch.randn(2, 8, 128, device="cuda") * size
+        out = attend(ctx, cache, q, scale=scale)
+        # a score of size S carries S * 2^-24 of absolute rounding into the softmax: S is up to 300 * 11 * 3 * 1.7
+        worst = (scale or 128 ** -0.5) * size * 11.3 * 5
+        close(out, reference(cache, q, scale or None)[0], F32, 1e-5 + worst * 2 ** -22)
+
+
+def test_attention_outliers(ctx):
+    """A few very large queries and keys beside small ones keep the small ones' precision."""
+    for dtype in (BF16, F16):
+        cache = Cache([200], 1, 8, 64, dtype, seed=5)
+        q = torch.randn(1, 4, 64, device="cuda")
+        q[0, 0, 3] = 1e4
+        q[0, 1] = 0
+        q[0, 2] *= 1e-30
+        pg, at = cache.cells(0, 200)
+        k = cache.k[pg, :, at]
+        k[:, :, 3] *= 1e-3
+        cache.k[pg, :, at] = k
+        close(attend(ctx, cache, q), reference(cache, q)[0], F32)
+
+
+@pytest.mark.parametrize("io", [F32, BF16])
+def test_attention_strides_and_alignment(ctx, io):
+    """Queries and outputs inside wider rows, off 16-byte boundaries; what lies between is left as it was."""
+    cache = Cache([90, 0, 33], 2, 16, 72, BF16, seed=6)
+    wide = torch.randn(3, 7, 75, device="cuda").to(io)
+    room = torch.full((3, 9, 81), 5.0, device="cuda").to(io)
+    q, out = wide[:, 1:5, 3:], room[:, 2:6, 1:73]
+    attend(ctx, cache, q, out)
+    close(out, reference(cache, q)[0], io)
+    room[:, 2:6, 1:73] = 5
+    assert (room == 5).all()
+    turned = torch.randn(4, 3, 72, device="cuda").to(io).transpose(0, 1)
+    close(attend(ctx, cache, turned, torch.empty_like(turned)), reference(cache, turned)[0], io)
+
+
+def test_attention_rows_that_share_pages(ctx):
+    """A window of candidates of one sequence: rows with the same pages and growing lengths."""
+    cache = Cache([100], 2, 16, 128, BF16, seed=7)
+    pages = cache.pages_dev.expand(5, -1).contiguous()
+    kv = mai.paged_kv(cache.k, cache.v, pages)
+    lengths = [96, 97, 98, 99, 100]
+    q = torch.randn(5, 8, 128, device="cuda")
+    out, n = torch.empty_like(q), torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    work = torch.empty(mai.paged_attention_workspace_bytes(kv, 8), dtype=torch.uint8, device="cuda")
+    ctx.paged_attention_dev(kv, mai.paged_attention(kv, q, out, n, work), LEGACY)
+    for i, m in enumerate(lengths):
+        cache.lengths = [m]
+        close(out[i:i + 1], reference(cache, q[i:i + 1])[0], F32)
+
+
+@pytest.mark.parametrize("g", [1, 4, 5, 11])
+@pytest.mark.parametrize("in_place", [True, False, None])
+def test_attention_weights(ctx, g, in_place):
+    """in_place None: no weights come in."""
+    lengths = [500, 0, 1, 17, 2000]
+    cache = Cache(lengths, 3, 16, 64, F16, seed=g, cols=150)
+    q = torch.randn(5, 3 * g, 64, device="cuda")
+    before = torch.rand(5, 3, 2048, device="cuda")
+    w_out = before.clone() if in_place else torch.full_like(before, 7.0)
+    w_in = w_out if in_place else None if in_place is None else before
+    out = attend(ctx, cache, q, weights_in=w_in, weights_out=w_out)
+    want, _, weights = reference(cache, q)
+    close(out, want, F32)
+    for b, n in enumerate(lengths):
+        rest = before if in_place else torch.full_like(before, 7.0)
+        assert torch.equal(w_out[b, :, n:], rest[b, :, n:])
+        if n:
+            start = before[b, :, :n].double() if in_place is not None else 0.0
+            close(w_out[b, :, :n], weights[b] + start, F32)
+    # the same call again gives the same bits
+    if in_place is False:
+        again = torch.full_like(before, 7.0)
+        assert torch.equal(attend(ctx, cache, q, weights_in=before, weights_out=again), out) and torch.equal(again, w_out)
+
+
+def test_attention_bad_pages_and_lengths(ctx):
+    """A page outside the pool is left out and reported, other rows stay right; so is a length beyond the table."""
+    cache = Cache([64, 64, 40], 2, 16, 64, BF16, seed=9)
+    q = torch.randn(3, 4, 64, device="cuda")
+    good = attend(ctx, cache, q)
+    ctx.synchronize()
+    for bad in (-1, cache.k.shape[0], 2 ** 31 - 1):
+        cache.pages_dev[1, 2] = bad
+        out = attend(ctx, cache, q)
+        torch.cuda.synchronize()
+        with pytest.raises(mai.SiError) as e:
+            ctx.synchronize()
+        assert e.value.status == mai.SI_E_INVALID
+        assert torch.equal(out[[0, 2]], good[[0, 2]]) and torch.isfinite(out).all()
+        left = torch.cat([torch.arange(32), torch.arange(48, 64)]).cuda()
+        k, v = (cache.rows(1, 64, p)[left] for p in (cache.k, cache.v))
+        p = torch.softmax(torch.einsum("hgd,nhd->hgn", q[1].double().view(2, 2, 64), k) / 8, -1)
+        close(out[1], torch.einsum("hgn,nhd->hgd", p, v).reshape(4, 64), F32)
+    cache.pages_dev.copy_(cache.pages)
+    for bad in (-5, 65, 2 ** 31 - 1):
+        cache.len_dev[1] = bad
+        out = attend(ctx, cache, q)
+        torch.cuda.synchronize()
+        with pytest.raises(mai.SiError):
+            ctx.synchronize()
+        assert torch.equal(out[[0, 2]], good[[0, 2]])
+        assert torch.equal(out[1], torch.zeros_like(out[1]) if bad < 0 else good[1])
+    ctx.synchronize()  # the report is given once
+
+
+def test_attention_far_offsets(ctx):
+    """Pools whose last page lies past 2^32 elements."""
+    stride = (1 << 31) + 1024
+    flat = [torch.empty(2 * stride + 4096, dtype=BF16, device="cuda") for _ in range(2)]
+    k, v = (f.as_strided((3, 1, 16, 64), (stride, 1024, 64, 1)) for f in flat)
+    k[...] = torch.randn(3, 1, 16, 64, device="cuda").to(BF16)
+    v[...] = torch.randn(3, 1, 16, 64, device="cuda").to(BF16)
+    pages = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    kv = mai.paged_kv(k, v, pages)
+    q = torch.randn(1, 2, 64, device="cuda")
+    out, n = torch.empty_like(q), torch.tensor([45], dtype=torch.int32, device="cuda")
+    work = torch.empty(mai.paged_attention_workspace_bytes(kv, 2), dtype=torch.uint8, device="cuda")
+    ctx.paged_attention_dev(kv, mai.paged_attention(kv, q, out, n, work), LEGACY)
+    keys, values = (x[[2, 0, 1], 0].reshape(48, 64)[:45].double() for x in (k, v))
+    close(out[0], torch.softmax(q[0].double() @ keys.T / 8, -1) @ values, F32)
+    # the append writes there too
+    new = torch.randn(1, 1, 64, device="cuda").to(BF16)
+    slot = torch.tensor([5], dtype=torch.int32, device="cuda")
+    ctx.paged_append_dev(kv, mai.paged_append(kv, None, new, new, None, slot), LEGACY)
+    assert torch.equal(k[2, 0, 5], new[0, 0]) and torch.equal(v[2, 0, 5], new[0, 0])
+
+
+def test_attention_captured_follows_lengths(ctx):
+    """A captured call replays with other lengths, pages and queries."""
+    cache = Cache([400, 3, 90], 2, 16, 128, BF16, seed=11)
+    q, s = torch.randn(3, 8, 128, device="cuda"), torch.cuda.Stream()
+    out, work = torch.empty_like(q), work_for(cache, 8)
+    args = mai.paged_attention(cache.desc, q, out, cache.len_dev, work)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        ctx.paged_attention_dev(cache.desc, args, s.cuda_stream)
+    for lengths in ([400, 3, 90], [1, 0, 17], [0, 0, 0], [399, 2, 80]):
+        cache.len_dev.copy_(torch.tensor(lengths))
+        q.normal_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        close(out, reference(cache, q, lengths=lengths)[0], F32)
+
+
+def test_attention_on_two_streams(ctx):
+    caches = [Cache([5000, 70], 4, 16, 128, BF16, seed=i) for i in (1, 2)]
+    qs = [torch.randn(2, 16, 128, device="cuda") for _ in caches]
+    outs, streams = [torch.empty_like(q) for q in qs], [torch.cuda.Stream() for _ in caches]
+    args = [mai.paged_attention(c.desc, q, o, c.len_dev, work_for(c, 16)) for c, q, o in zip(caches, qs, outs)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, a, s in zip(caches, args, streams):
+            ctx.paged_attention_dev(c.desc, a, s.cuda_stream)
+    torch.cuda.synchronize()
+    for c, q, o in zip(caches, qs, outs):
+        close(o, reference(c, q)[0], F32)
+
+
+# ---- rotary positions and append ------------------------------------------------
+def rotated(x, angle, layout, scale):
+    half = angle.shape[1]
+    y = x.double().clone()
+    c, s = (f(angle)[:, None] * scale for f in (torch.cos, torch.sin))
+    if layout == "half":
+        a, b = x[..., :half].double(), x[..., half:2 * half].double()
+        y[..., :half], y[..., half:2 * half] = a * c - b * s, a * s + b * c
+    else:
+        a, b = x[..., :2 * half:2].double(), x[..., 1:2 * half:2].double()
+        y[..., :2 * half:2], y[..., 1:2 * half:2] = a * c - b * s, a * s + b * c
+    return y
+
+
+APPEND = [
+    # tokens, sequences, query heads, kv heads, head_dim, rotary, page
+    (1, 1, 4, 4, 64, 64, 1),
+    (5, 5, 24, 4, 256, 64, 16),
+    (77, 3, 6, 2, 128, 128, 24),
+    (40, 2, 3, 1, 80, 20, 7),
+    (33, 4, 2, 2, 72, 2, 16),
+    (6, 6, 8, 8, 96, 0, 8),
+    (2000, 7, 4, 2, 64, 48, 32),
+    (5000, 2, 5, 1, 8, 8, 5),
+]
+
+
+@pytest.mark.parametrize("io, cache_type", [(F32, BF16), (BF16, BF16), (F16, F16), (F32, F16), (BF16, F16)])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("case", range(len(APPEND)))
+def test_append(ctx, case, layout, io, cache_type):
+    tokens, seqs, qh, kvh, hd, rotary, page = APPEND[case]
+    gen = torch.Generator().manual_seed(case)
+    per = -(-tokens // seqs)
+    cache = Cache([per + 3] * seqs, kvh, page, hd, cache_type, seed=case)
+    order = torch.randperm(tokens, generator=gen)
+    sequence, slot = (order // per).to(torch.int32), (order % per + 2).to(torch.int32)
+    position = torch.randint(-1000, 1 << 20, (tokens,), generator=gen, dtype=torch.int32)
+    position[0] = 2 ** 31 - 1
+    pad = torch.rand(tokens, generator=gen) < 0.1
+    slot[pad] = -1
+    qkv = torch.randn(tokens, qh + 2 * kvh, hd, generator=gen).to(io).cuda()
+    q, k, v = qkv.split([qh, kvh, kvh], 1)
+    kind = ["none", "linear", "ntk", "yarn", "banded"][case % 5]
+    table, scale = mai.rope_table(1e6, rotary, kind, factor=4.0, original=4096)
+    rope = torch.from_numpy(table.view(np.int64)).cuda()
+    q_out = torch.full_like(q.contiguous(), 9.0)
+    want_k, want_v = cache.k.clone(), cache.v.clone()
+    args = mai.paged_append(cache.desc, q, k, v, q_out, slot.cuda(), sequence=sequence.cuda(), position=position.cuda(),
+                            rope=rope, rotary_dim=rotary, layout=layout, rope_scale=scale)
+    ctx.paged_append_dev(cache.desc, args, LEGACY)
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    # exact angles: integer turns modulo 2^64, from the table itself
+    turns = [[(int(p) * int(t)) % 2 ** 64 / 2.0 ** 64 * 2 * math.pi for t in table] for p in position]
+    angle = torch.tensor(turns, dtype=torch.float64).view(tokens, rotary // 2).cuda()
+    live = ~pad.cuda()
+
+    def check(got, x, dtype):
+        """2^-24 for each of three roundings, 2^-22 for the sines and the angle, of |x| + |y| <= 1.5 max"""
+        want = rotated(x, angle, layout, scale)
+        room = x.double().abs().amax(-1, keepdim=True) * 2 * scale * 2 ** -21 + want.abs() * half_step(dtype)
+        if dtype == F16:
+            room = room + 2 ** -25  # half a step of the subnormal range
+        assert ((got.double() - want).abs() <= room)[live].all()
+
+    check(q_out, q, io)
+    assert (q_out[~live] == 9).all()
+    pg = cache.pages_dev.long()[sequence.long().cuda(), (slot.long().clamp(min=0) // page).cuda()]
+    at = (slot.long().clamp(min=0) % page).cuda()
+    check(cache.k[pg, :, at], k, cache_type)
+    new_v = v.to(F32).to(cache_type)
+    assert torch.equal(cache.v[pg, :, at][live], new_v[live])
+    # nothing else changed
+    cache.k[pg[live], :, at[live]] = 0
+    cache.v[pg[live], :, at[live]] = 0
+    want_k[pg[live], :, at[live]] = 0
+    want_v[pg[live], :, at[live]] = 0
+    assert torch.equal(cache.k.view(torch.int16), want_k.view(torch.int16))
+    assert torch.equal(cache.v.view(torch.int16), want_v.view(torch.int16))
+
+
+def test_append_in_place_defaults_and_parts(ctx):
+    """Queries in place, token t of sequence t, position = slot; queries only; keys only; off 16-byte boundaries."""
+    cache = Cache([20, 20, 20], 2, 8, 64, BF16, seed=1)
+    table, _ = mai.rope_table(1e4, 64)
+    rope = torch.from_numpy(table.view(np.int64)).cuda()
+    slot = torch.tensor([19, -1, 4], dtype=torch.int32, device="cuda")
+    angle = torch.tensor([[int(p) * int(t) / 2.0 ** 64 * 2 * math.pi for t in table] for p in slot], dtype=torch.float64).cuda()
+    big = torch.randn(3, 5, 67, device="cuda")
+    q = big[:, :, 2:66]
+    before = q.clone()
+    ctx.paged_append_dev(cache.desc, mai.paged_append(cache.desc, q, None, None, q, slot, rope=rope, rotary_dim=64), LEGACY)
+    want = rotated(before, angle, "interleaved", 1.0)
+    want[1] = before[1]
+    close(q, want, F32)
+    kept = cache.k.clone()
+    new = torch.randn(3, 2, 64, device="cuda").to(BF16)
+    ctx.paged_append_dev(cache.desc, mai.paged_append(cache.desc, None, new, new, None, slot, rope=rope, rotary_dim=64, layout="half"),
+                         LEGACY)
+    for b, t in ((0, 19), (2, 4)):
+        got = cache.k[cache.pages[b, t // 8].item(), :, t % 8]
+        close(got, rotated(new[b:b + 1], angle[b:b + 1], "half", 1.0)[0], BF16)
+        assert torch.equal(cache.v[cache.pages[b, t // 8].item(), :, t % 8], new[b])
+        cache.k[cache.pages[b, t // 8].item(), :, t % 8] = kept[cache.pages[b, t // 8].item(), :, t % 8]
+    assert torch.equal(cache.k.view(torch.int16), kept.view(torch.int16))
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    empty = torch.zeros(0, 2, 64, device="cuda")
+    ctx.paged_append_dev(cache.desc, mai.paged_append(cache.desc, None, empty, empty, None, none), LEGACY)
+    ctx.synchronize()
+
+
+def test_append_bad_places_are_left_out(ctx):
+    cache = Cache([16, 16], 1, 8, 64, BF16, seed=2)
+    cache.pages_dev[1, 1] = cache.k.shape[0]
+    k0, v0 = cache.k.clone(), cache.v.clone()
+    new = torch.randn(4, 1, 64, device="cuda").to(BF16)
+    slot = torch.tensor([16, 9, 3, 0], dtype=torch.int32, device="cuda")      # beyond the table, a bad page, good,
+    sequence = torch.tensor([0, 1, 0, 2], dtype=torch.int32, device="cuda")   # no such sequence
+    ctx.paged_append_dev(cache.desc, mai.paged_append(cache.desc, None, new, new, None, slot, sequence=sequence), LEGACY)
+    torch.cuda.synchronize()
+    with pytest.raises(mai.SiError) as e:
+        ctx.synchronize()
+    assert e.value.status == mai.SI_E_INVALID
+    pg = cache.pages[0, 0].item()
+    assert torch.equal(cache.k[pg, :, 3], new[2])
+    cache.k[pg, :, 3], cache.v[pg, :, 3] = k0[pg, :, 3], v0[pg, :, 3]
+    assert torch.equal(cache.k.view(torch.int16), k0.view(torch.int16))
+    assert torch.equal(cache.v.view(torch.int16), v0.view(torch.int16))
+
+
+# ---- eviction -----------------------------------------------------------------------
+def evicted(w, pos, n, budget, sink, recent, nxt):
+    """(holes, kept slots behind the budget) of one row: the definition, by sorting."""
+    m = min(n, budget)
+    key = []
+    for t in range(n):
+        held = pos[t] < sink or pos[t] >= nxt - recent
+        x = float(w[t])
+        key.append((1 if held else 0, 0.0 if held else (-math.inf if x != x else x), 0 if x != x or held else 1, t))
+    gone = {k[-1] for k in sorted(key)[:n - m]}
+    return [t for t in range(m) if t in gone], [t for t in range(m, n) if t not in gone]
+
+
+EVICT = [
+    # lengths, kv_heads, head_dim, page, budget, sink, recent
+    ([1], 1, 64, 1, 1, 0, 0),
+    ([2, 0, 1], 2, 8, 4, 1, 0, 1),
+    ([100, 20, 0, 21, 300], 2, 64, 16, 20, 2, 5),
+    ([500], 3, 256, 24, 499, 4, 100),
+    ([1023, 1024, 1025], 2, 128, 64, 512, 0, 512),
+    ([5000, 40], 1, 72, 7, 33, 3, 30),
+    ([9000, 17000], 2, 64, 32, 4000, 4, 64),
+    ([40000], 1, 8, 256, 20001, 1, 1),
+    ([70001, 3], 1, 8, 128, 100, 50, 50),
+    ([200], 2, 64, 16, 1000, 0, 0),
+]
+
+
+@pytest.mark.parametrize("kind", ["spread", "ties", "equal", "strange"])
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("case", range(len(EVICT)))
+def test_evict(ctx, case, in_place, kind):
+    lengths, kvh, hd, page, budget, sink, recent = EVICT[case]
+    rng = np.random.default_rng(case)
+    cache = Cache(lengths, kvh, page, hd, F16 if case % 2 else BF16, order="tokens_first" if case % 3 else "heads_first", seed=case)
+    width = max(lengths) + 5
+    shape = (len(lengths), kvh, width)
+    w = np.exp(3 * rng.normal(size=shape)).astype(np.float32)
+    if kind == "ties":
+        w = np.floor(w * 4) / 4
+    elif kind == "equal":
+        w[:] = 0.5
+    elif kind == "strange":
+        odd = rng.random(shape)
+        w[odd < 0.1] = np.nan
+        w[(odd >= 0.1) & (odd < 0.2)] = np.inf
+        w[(odd >= 0.2) & (odd < 0.3)] = -np.inf
+        w[(odd >= 0.3) & (odd < 0.5)] *= -1
+        w[(odd >= 0.5) & (odd < 0.6)] = 0.0
+        w[(odd >= 0.6) & (odd < 0.7)] = -0.0
+    w = w.astype(np.float32)
+    pos = np.stack([np.stack([rng.permutation(width * 2)[:width] for _ in range(kvh)]) for _ in lengths]).astype(np.int32)
+    nxt = np.array([2 * width] * len(lengths), np.int32)
+    w_in, p_in = torch.from_numpy(w).cuda(), torch.from_numpy(pos).cuda()
+    w_out = w_in.clone() if in_place else torch.full_like(w_in, 3.5)
+    p_out = p_in.clone() if in_place else torch.full_like(p_in, -9)
+    n_out = cache.len_dev.clone() if in_place else torch.full_like(cache.len_dev, -1)
+    work = torch.empty(mai.paged_evict_workspace_bytes(cache.desc), dtype=torch.uint8, device="cuda").fill_(255)
+    k0, v0 = cache.k.clone(), cache.v.clone()
+    args = mai.paged_evict(cache.desc, n_out if in_place else cache.len_dev, n_out, w_out if in_place else w_in, w_out,
+                           budget, work, sink=sink, recent=recent, positions_in=p_out if in_place else p_in,
+                           positions_out=p_out, next_position=torch.from_numpy(nxt).cuda())
+    ctx.paged_evict_dev(cache.desc, args, LEGACY)
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    assert n_out.tolist() == [min(n, budget) for n in lengths]
+    want_w = w.copy() if in_place else np.full_like(w, 3.5)
+    want_p = pos.copy() if in_place else np.full_like(pos, -9)
+    for b, n in enumerate(lengths):
+        m = min(n, budget)
+        for h in range(kvh):
+            holes, movers = evicted(w[b, h], pos[b, h], n, budget, sink, recent, nxt[b])
+            keep = [t for t in range(m) if t not in set(holes)]
+            want_w[b, h, keep], want_p[b, h, keep] = w[b, h, keep], pos[b, h, keep]
+            want_w[b, h, holes], want_p[b, h, holes] = w[b, h, movers], pos[b, h, movers]
+            if holes:
+                pg, at = cache.cells(b, n)
+                to, of = torch.tensor(holes).cuda(), torch.tensor(movers).cuda()
+                for pool, start in ((cache.k, k0), (cache.v, v0)):
+                    assert torch.equal(pool[pg[to], h, at[to]], start[pg[of], h, at[of]])
+                    pool[pg[to], h, at[to]] = start[pg[to], h, at[to]]
+    if not in_place:  # holes of the output are written, slots behind the new length are not
+        for b, n in enumerate(lengths):
+            assert (w_out[b, :, min(n, budget):] == 3.5).all()
+    np.testing.assert_array_equal(w_out.cpu().numpy().view(np.uint32), want_w.view(np.uint32))
+    np.testing.assert_array_equal(p_out.cpu().numpy(), want_p)
+    assert torch.equal(cache.k.view(torch.int16), k0.view(torch.int16))
+    assert torch.equal(cache.v.view(torch.int16), v0.view(torch.int16))
+
+
+def test_evict_without_positions(ctx):
+    """Slots are positions: the first `sink` and the last `recent` slots stay, and the positions come out."""
+    cache = Cache([50, 9], 1, 8, 64, BF16, seed=3)
+    w = torch.rand(2, 1, 64, device="cuda")
+    w[0, 0, 10] = w[0, 0, 3] = 0.0
+    p_out = torch.full((2, 1, 64), -1, dtype=torch.int32, device="cuda")
+    n_out, w_out = torch.empty_like(cache.len_dev), w.clone()
+    work = torch.empty(mai.paged_evict_workspace_bytes(cache.desc), dtype=torch.uint8, device="cuda")
+    args = mai.paged_evict(cache.desc, cache.len_dev, n_out, w_out, w_out, 48, work, sink=2, recent=5, positions_out=p_out)
+    ctx.paged_evict_dev(cache.desc, args, LEGACY)
+    assert n_out.tolist() == [48, 9]
+    want = list(range(48))
+    want[3], want[10] = 48, 49
+    assert p_out[0, 0, :48].tolist() == want and p_out[1, 0, :9].tolist() == list(range(9))
+    assert (p_out[0, 0, 48:] == -1).all() and (p_out[1, 0, 9:] == -1).all()
+
+
+def test_evict_bad_pages_lengths_and_too_many_protected(ctx):
+    cache = Cache([64, 64], 1, 16, 64, BF16, seed=4)
+    w = torch.rand(2, 1, 64, device="cuda")
+    w[:, :, :8] = 0
+    work = torch.empty(mai.paged_evict_workspace_bytes(cache.desc), dtype=torch.uint8, device="cuda")
+    k0 = cache.k.clone()
+    cache.pages_dev[0, 3] = -3  # where the kept slots lie
+    n_out = torch.empty_like(cache.len_dev)
+    ctx.paged_evict_dev(cache.desc, mai.paged_evict(cache.desc, cache.len_dev, n_out, w, w.clone(), 56, work, recent=8), LEGACY)
+    torch.cuda.synchronize()
+    with pytest.raises(mai.SiError) as e:
+        ctx.synchronize()
+    assert e.value.status == mai.SI_E_INVALID
+    pg = cache.pages[1].long().cuda()
+    assert torch.equal(cache.k[pg[0], 0, :8], k0[pg[3], 0, 8:])  # the other sequence moved
+    assert torch.equal(cache.k[cache.pages[0, 0].item()].view(torch.int16), k0[cache.pages[0, 0].item()].view(torch.int16))
+    cache.pages_dev.copy_(cache.pages)
+    for bad in (65, -1):
+        cache.len_dev[0] = bad
+        ctx.paged_evict_dev(cache.desc, mai.paged_evict(cache.desc, cache.len_dev, n_out, w, w.clone(), 56, work, recent=8), LEGACY)
+        torch.cuda.synchronize()
+        with pytest.raises(mai.SiError):
+            ctx.synchronize()
+        assert n_out.tolist() == [56 if bad > 0 else 0, 56]
+    # all positions are protected: the lowest slots leave
+    cache = Cache([20], 1, 16, 64, BF16, seed=4)
+    p = torch.zeros(1, 1, 32, dtype=torch.int32, device="cuda")
+    p_out, n_out = torch.empty_like(p), torch.empty_like(cache.len_dev)
+    p[0, 0, 16:20] = torch.arange(-4, 0)
+    w = torch.rand(1, 1, 32, device="cuda")
+    ctx.paged_evict_dev(cache.desc, mai.paged_evict(cache.desc, cache.len_dev, n_out, w, w, 16, work, sink=16, positions_in=p,
+                                                    positions_out=p_out), LEGACY)
+    assert p_out[0, 0, :16].tolist() == [-4, -3, -2, -1] + [0] * 12
+
+
+# ---- verification ------------------------------------------------------------------------
+def verified(p, q, tokens, u, last, n):
+    """The definition, in exact rational arithmetic up to the 64-bit sums."""
+    good = lambda x: x if 0 < x < math.inf else 0.0  # noqa: E731
+    i = 0
+    while i < n:
+        x = int(tokens[i])
+        if not 0 <= x < p.shape[1]:
+            break
+        if not float(u[i]) * (good(float(q[i, x])) if q is not None else 1.0) < good(float(p[i, x])):
+            break
+        i += 1
+    clean = lambda a: np.where((a > 0) & np.isfinite(a), a, 0).astype(np.float64)  # noqa: E731
+    row = clean(p[i])
+    rest = row.copy()
+    if i < n:
+        if q is not None:
+            rest = np.maximum(row - clean(q[i]), 0)
+        elif 0 <= int(tokens[i]) < len(row):
+            rest[int(tokens[i])] = 0
+    if not rest.sum() > 0:
+        rest = row
+    if not rest.sum() > 0:
+        return i, -1
+    cdf = np.cumsum(rest)
+    hit = np.flatnonzero((cdf > float(last) * cdf[-1]) & (rest > 0))
+    return i, int(hit[0] if len(hit) else np.flatnonzero(rest)[-1])
+
+
+def run_verify(ctx, p, q, tokens, u, last, counts=None, stream=LEGACY):
+    n = p.shape[0]
+    accepted, following = (torch.full((n,), -5, dtype=torch.int32, device="cuda") for _ in range(2))
+    work = torch.empty(mai.verify_drafts_workspace_bytes(n, p.shape[2]), dtype=torch.uint8, device="cuda").fill_(255)
+    args = mai.verify_drafts(p, tokens, u, last, accepted, following, work, draft_probs=q, counts=counts)
+    ctx.verify_drafts_dev(args, stream)
+    return accepted, following
+
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("n, k, vocab", [(1, 0, 1), (1, 1, 1), (5, 3, 2), (7, 8, 257), (3, 32, 4096), (4, 4, 4097), (9, 2, 32003),
+                                         (2, 7, 248320), (300, 1, 100)])
+def test_verify(ctx, n, k, vocab, probs):
+    gen = torch.Generator(device="cuda").manual_seed(n * k + vocab)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    logits = 2 * rnd(n, k + 1, vocab)
+    p = torch.softmax(logits, -1)
+    q = torch.softmax(logits[:, :k] + 0.5 * rnd(n, k, vocab), -1) if probs else None
+    tokens = torch.randint(0, vocab, (n, k), device="cuda", generator=gen, dtype=torch.int32)
+    if k:
+        tokens = torch.where(torch.rand(n, k, device="cuda", generator=gen) < 0.8, p[:, :k].argmax(-1).to(torch.int32), tokens)
+    u, last = torch.rand(n, k, device="cuda", generator=gen), torch.rand(n, device="cuda", generator=gen)
+    last[0] = 0.0
+    if n > 2:
+        last[1] = 1 - 2 ** -24
+    counts = torch.randint(0, k + 1, (n,), device="cuda", generator=gen, dtype=torch.int32)
+    for c in (None, counts):
+        accepted, following = run_verify(ctx, p, q, tokens, u, last, c)
+        ctx.synchronize()
+        for b in range(n):
+            want = verified(p[b].cpu().numpy(), q[b].cpu().numpy() if probs else None, tokens[b].tolist(), u[b].tolist(),
+                            last[b].item(), k if c is None else int(c[b]))
+            assert (accepted[b].item(), following[b].item()) == want, b
+
+
+def test_verify_edges(ctx):
+    """Equal rows, empty rows, values on the border, entries that are no probabilities, drafts outside the vocabulary."""
+    p = torch.zeros(9, 2, 6, device="cuda")
+    q = torch.zeros(9, 1, 6, device="cuda")
+    tokens, u, last = torch.zeros(9, 1, dtype=torch.int32, device="cuda"), torch.zeros(9, 1, device="cuda"), torch.full((9,), 0.5, device="cuda")
+    p[0, 0], q[0, 0], tokens[0] = torch.tensor([0, .5, .5, 0, 0, 0]), torch.tensor([0, .5, .5, 0, 0, 0]), 0  # 0 < 0: rejected; p - q is 0: p itself
+    p[1, 0, 2], q[1, 0, 2], tokens[1], u[1] = 0.25, 0.5, 2, 0.5        # u q == p: rejected
+    p[2, 0, 2], q[2, 0, 2], tokens[2], u[2] = 0.25, 0.5, 2, 0.49999997  # below: accepted
+    p[2, 1, 5] = 1.0
+    p[3, 0] = math.nan                                                  # nothing to draw: -1
+    p[4, 0], tokens[4] = torch.tensor([math.nan, -1, math.inf, 0, .5, .5]), 0
+    p[5, 0], tokens[5], u[5] = torch.tensor([.2, .2, .2, .2, .2, 0]), 4, 0.9
+    q[5, 0] = torch.tensor([.1, .2, .3, .1, .3, 0])                     # left: .1 at 0 and 3
+    p[6, 0, 1], p[6, 0, 3], tokens[6] = .5, .5, -1                      # outside: rejected, reported
+    p[7, 0, 1], p[7, 0, 3], tokens[7] = .5, .5, 6
+    p[8, 0, 0], q[8, 0, 0], p[8, 1, 3] = 1.0, 1.0, 1e-45                # accepted; a subnormal row
+    accepted, following = run_verify(ctx, p, q, tokens, u, last)
+    torch.cuda.synchronize()
+    with pytest.raises(mai.SiError) as e:
+        ctx.synchronize()
+    assert e.value.status == mai.SI_E_INVALID
+    assert accepted.tolist() == [0, 0, 1, 0, 0, 0, 0, 0, 1]
+    # half of equal halves: the lowest whose sum passes 0.5 is the second
+    assert following.tolist() == [2, 2, 5, -1, 5, 3, 3, 3, 3]
+    last[0] = 0.0
+    assert run_verify(ctx, p, q, tokens, u, last)[1][0].item() == 1
+    torch.cuda.synchronize()
+    with pytest.raises(mai.SiError):
+        ctx.synchronize()
+
+
+def test_verify_strides_capture_and_shared_rows(ctx):
+    """Rows inside wider ones (a logits buffer with padding), captured and replayed on a stream of its own."""
+    wide_p, wide_q = torch.rand(3, 4, 1003, device="cuda"), torch.rand(3, 3, 1010, device="cuda")
+    p, q = wide_p[:, :, 1:1001], wide_q[:, :, 5:1005]
+    tokens = torch.randint(0, 1000, (3, 3), device="cuda", dtype=torch.int32)
+    u, last = torch.rand(3, 3, device="cuda"), torch.rand(3, device="cuda")
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    accepted, following = torch.empty(3, dtype=torch.int32, device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda")
+    work = torch.empty(mai.verify_drafts_workspace_bytes(3, 1000), dtype=torch.uint8, device="cuda")
+    args = mai.verify_drafts(p, tokens, u, last, accepted, following, work, draft_probs=q)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        ctx.verify_drafts_dev(args, s.cuda_stream)
+    for _ in range(4):
+        wide_p.uniform_(), u.uniform_(), last.uniform_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for b in range(3):
+            assert (accepted[b].item(), following[b].item()) == verified(p[b].cpu().numpy(), q[b].cpu().numpy(), tokens[b].tolist(),
+                                                                         u[b].tolist(), last[b].item(), 3)
+
+
+# ---- the operators together ----------------------------------------------------------------
+def test_a_bounded_cache_from_prompt_to_eviction(ctx):
+    """Two sequences: prompts appended in chunks, then steps that append, attend with weights, and evict to a
+    budget, all enqueued without a wait; a plain 64-bit cache that never moves anything follows along."""
+    kvh, g, hd, page, budget, sink, recent = 2, 3, 64, 8, 40, 2, 8
+    prompts, steps = [45, 13], 30
+    cache = Cache([56, 56], kvh, page, hd, BF16, seed=8)
+    table, scale = mai.rope_table(1e4, 32, "yarn", factor=4.0, original=64)
+    rope = torch.from_numpy(table.view(np.int64)).cuda()
+    weights = torch.zeros(2, kvh, 56, device="cuda")
+    positions = torch.zeros(2, kvh, 56, dtype=torch.int32, device="cuda")
+    length = torch.tensor(prompts, dtype=torch.int32, device="cuda")
+    evict_work = torch.empty(mai.paged_evict_workspace_bytes(cache.desc), dtype=torch.uint8, device="cuda")
+    kept = [[{} for _ in range(kvh)] for _ in range(2)]  # position -> (key, value, weight)
+    # prompt
+    rows = [(b, t) for b, n in enumerate(prompts) for t in range(n)]
+    seq, slot = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in zip(*rows))
+    k, v = (torch.randn(len(rows), kvh, hd, device="cuda") for _ in range(2))
+    for lo in range(0, len(rows), 25):
+        part = slice(lo, lo + 25)
+        ctx.paged_append_dev(cache.desc, mai.paged_append(cache.desc, None, k[part], v[part], None, slot[part].contiguous(),
+                                                          sequence=seq[part].contiguous(), rope=rope, rotary_dim=32, layout="half",
+                                                          rope_scale=scale), LEGACY)
+    positions[:] = torch.arange(56, dtype=torch.int32, device="cuda")
+    turned = rotated(k, slot.double()[:, None] * torch.tensor(table.astype(np.float64) / 2.0 ** 64 * 2 * math.pi).cuda(), "half", scale)
+    for i, (b, t) in enumerate(rows):
+        for h in range(kvh):
+            kept[b][h][t] = [turned[i, h].to(BF16).double(), v[i, h].to(BF16).double(), 0.0]
+    seen = list(prompts)
+    for step in range(steps):
+        q = torch.randn(2, kvh * g, hd, device="cuda")
+        k, v = (torch.randn(2, kvh, hd, device="cuda") for _ in range(2))
+        position = torch.tensor(seen, dtype=torch.int32, device="cuda")
+        slot = length.clone()
+        q_rot, out = torch.empty_like(q), torch.empty_like(q)
+        ctx.paged_append_dev(cache.desc, mai.paged_append(cache.desc, q, k, v, q_rot, slot, position=position, rope=rope,
+                                                          rotary_dim=32, layout="half", rope_scale=scale), LEGACY)
+        at = slot.long()[:, None].expand(2, kvh)[..., None]
+        positions.scatter_(2, at, position[:, None, None].expand(2, kvh, 1).contiguous())
+        weights.scatter_(2, at, 0.0)
+        length += 1
+        work = work_for(cache, kvh * g, True)
+        ctx.paged_attention_dev(cache.desc, mai.paged_attention(cache.desc, q_rot, out, length, work, weights_in=weights,
+                                                                weights_out=weights), LEGACY)
+        nxt = position + 1
+        ctx.paged_evict_dev(cache.desc, mai.paged_evict(cache.desc, length, length, weights, weights, budget, evict_work, sink=sink,
+                                                        recent=recent, positions_in=positions, positions_out=positions,
+                                                        next_position=nxt), LEGACY)
+        angle = position.double()[:, None] * torch.tensor(table.astype(np.float64) / 2.0 ** 64 * 2 * math.pi).cuda()
+        kr, qr = rotated(k, angle, "half", scale), rotated(q, angle, "half", scale)
+        for b in range(2):
+            want = torch.zeros(kvh * g, hd, dtype=torch.float64, device="cuda")
+            for h in range(kvh):
+                kept[b][h][seen[b]] = [kr[b, h].to(BF16).double(), v[b, h].to(BF16).double(), 0.0]
+                order = sorted(kept[b][h])
+                keys, values = (torch.stack([kept[b][h][p][i] for p in order]) for i in (0, 1))
+                prob = torch.softmax(qr[b, h * g:(h + 1) * g] @ keys.T / 8, -1)
+                want[h * g:(h + 1) * g] = prob @ values
+                for p, x in zip(order, prob.sum(0).tolist()):
+                    kept[b][h][p][2] += x
+                free = sorted((p for p in order if sink <= p < seen[b] + 1 - recent), key=lambda p: kept[b][h][p][2])
+                for p in free[:max(0, len(order) - budget)]:
+                    del kept[b][h][p]
+            # keys rounded from f32 and from f64 rotations differ by a bf16 step now and then: 2^-8 of one product
+            close(out[b], want, F32, 1e-3)
+            seen[b] += 1
+    ctx.synchronize()
+    assert length.tolist() == [min(n + steps, budget) for n in prompts]
+    for b in range(2):
+        n = length[b].item()
+        for h in range(kvh):
+            got = positions[b, h, :n].tolist()
+            assert len(set(got)) == n and set(got) == set(kept[b][h])
+            assert all(abs(weights[b, h, i].item() - kept[b][h][p][2]) < 1e-2 for i, p in enumerate(got))
+
+
+def test_drafts_over_the_paged_cache(ctx):
+    """A window of drafts as rows that share pages: probabilities from attention rows, verification, and the cache
+    kept to the accepted tokens by the length alone."""
+    kvh, g, hd, page, k_drafts, vocab = 2, 2, 64, 8, 3, 97
+    cache = Cache([30], kvh, page, hd, BF16, seed=12, room=2)
+    pages = cache.pages_dev.expand(k_drafts + 1, -1).contiguous()
+    kv = mai.paged_kv(cache.k, cache.v, pages)
+    new_k, new_v = (torch.randn(k_drafts + 1, kvh, hd, device="cuda") for _ in range(2))
+    slot = torch.arange(30, 31 + k_drafts, dtype=torch.int32, device="cuda")
+    ctx.paged_append_dev(kv, mai.paged_append(kv, None, new_k, new_v, None, slot), LEGACY)
+    q = torch.randn(k_drafts + 1, kvh * g, hd, device="cuda")
+    out, n = torch.empty_like(q), slot + 1
+    work = torch.empty(mai.paged_attention_workspace_bytes(kv, kvh * g), dtype=torch.uint8, device="cuda")
+    ctx.paged_attention_dev(kv, mai.paged_attention(kv, q, out, n, work), LEGACY)
+    for i in range(k_drafts + 1):
+        cache.lengths = [31 + i]
+        close(out[i:i + 1], reference(cache, q[i:i + 1])[0], F32)
+    head = torch.randn(kvh * g * hd, vocab, device="cuda") / 8
+    p = torch.softmax(out.reshape(k_drafts + 1, -1) @ head, -1)[None]
+    tokens = p[:, :k_drafts].argmax(-1).to(torch.int32)
+    u, last = torch.tensor([[0.0, 0.9999999, 0.0]], device="cuda"), torch.tensor([0.3], device="cuda")
+    accepted, following = run_verify(ctx, p, None, tokens, u, last)
+    want = verified(p[0].cpu().numpy(), None, tokens[0].tolist(), u[0].tolist(), 0.3, k_drafts)
+    assert (accepted.item(), following.item()) == (want[0], verified(p[0].cpu().numpy(), None, tokens[0].tolist(), u[0].tolist(),
+                                                                     last.item(), k_drafts)[1])
+    ctx.synchronize()
