@@ -131,7 +131,8 @@ int si_paged_append_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_appen
  * of length 0 gets zeros (and lse = -inf): rows of a padded batch have length
  * 0. Cached values at slots in use are taken to be finite; whatever lies in
  * other slots is not read. Sums and the softmax are held in f32, with f32
- * queries and f32 output the products too.
+ * queries and f32 output the products too. The same call gives the same bits;
+ * how the sums group depends on all lengths of the batch.
  * With weights_out, weights_out[b][h][t] = weights_in[b][h][t] + the sum of
  * the probabilities of slot t over the query heads of kv head h, for
  * t < lengths[b]; other entries are left as they are. weights_in may be

@@ -37,7 +37,7 @@
 // each multiplied separately into the same f32 accumulators. 16-bit queries of
 // the cache's own type are exact in one term. f32 queries take 3 bf16 terms
 // (24 bits) or 2 f16 terms (22 bits, after scaling each query by a power of two
-// to a maximum near 1), probabilities 3 bf16 or 2 f16 terms with f32 output and
+// to a maximum near 2^15), probabilities 3 bf16 or 2 f16 terms with f32 output and
 // 2 with 16-bit output. In f16, probabilities are scaled by 2^15 so that small ones keep
 // their bits; the sum is taken of the same scaled values.
 #include <cuda_runtime.h>
@@ -265,11 +265,11 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
 #pragma unroll
         for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(q[s][j]));
       }
-      if constexpr (!BF16) {  // to a maximum in [1, 2): f16 has no exponent to spare
+      if constexpr (!BF16) {  // to a maximum in [2^14, 2^15): small elements beside large ones keep their bits
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         int e = 0;
-        if (big > 0.f && big < INFINITY) e = max(-100, ilogbf(big));
+        if (big > 0.f && big < INFINITY) e = max(-100, ilogbf(big)) - 14;
         const float down = ldexpf(1.f, -e);
         col_scale *= ldexpf(1.f, e);
 #pragma unroll

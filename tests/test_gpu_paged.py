@@ -246,7 +246,9 @@ def test_attention_bad_pages_and_lengths(ctx):
         torch.cuda.synchronize()
         with pytest.raises(mai.SiError):
             ctx.synchronize()
-        assert torch.equal(out[[0, 2]], good[[0, 2]])
+        # another length shares the units out differently, so sums of the same terms group differently: 64 terms
+        # of 2^-24 each stay within 2^-18 of the largest value, inside the f32 bound
+        close(out[[0, 2]], good[[0, 2]], F32)
         assert torch.equal(out[1], torch.zeros_like(out[1]) if bad < 0 else good[1])
     ctx.synchronize()  # the report is given once
 
