@@ -60,7 +60,7 @@ typedef struct si_paged_kv {
   uint32_t elem;            /* SI_ELEM_BF16 or SI_ELEM_F16 */
   uint32_t kv_heads, head_dim; /* head_dim: a multiple of 8, at most 256 */
   uint32_t page_tokens;     /* any number from 1 */
-  uint32_t sequences;       /* at most 8192 */
+  uint32_t sequences;       /* at most 4096 */
   uint32_t max_pages;       /* page_tokens * max_pages below 2^31 */
 } si_paged_kv;
 /* Host only: where slot `slot` of a sequence whose page is `page` lies in a

@@ -22,7 +22,7 @@ int check_paged_kv(const si_paged_kv* kv, std::string* msg) {
     return bad(SI_E_INVALID, "paged cache sizes must be positive");
   if (kv->num_pages > 0x7fffffffull || uint64_t(kv->page_tokens) * kv->max_pages > 0x7fffffffull)
     return bad(SI_E_UNSUPPORTED, "paged cache pages and slots must be below 2^31");
-  if (kv->sequences > 8192) return bad(SI_E_UNSUPPORTED, "a paged cache call takes at most 8192 sequences");
+  if (kv->sequences > 4096) return bad(SI_E_UNSUPPORTED, "a paged cache call takes at most 4096 sequences");
   if (uint64_t(kv->sequences) * ((uint64_t(kv->page_tokens) * kv->max_pages + 15) / 16) > 0xffffffffull)
     return bad(SI_E_UNSUPPORTED, "paged cache page table spans too many slots");
   if (kv->pages_stride < kv->max_pages)

@@ -52,6 +52,9 @@ namespace {
 
 constexpr uint32_t kUnit = 16;  // slots of a unit
 constexpr uint32_t kCols = 8;   // query heads of a block
+// Beginning a pair (its queries, its first pages) and ending it costs a warp
+// about as much time as this many units; shares are even in that measure.
+constexpr uint32_t kPairCost = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -63,7 +66,7 @@ struct Shape {
 
 // Join records and partials in the workspace (one CTA: two partial slots).
 struct Join {
-  int32_t last;    // last CTA of the pair that crosses this CTA's first border; -1: none starts before it
+  int32_t last;    // last CTA of the pair that crosses this CTA's first border; -1: none whose first border it is
   uint32_t slot0;  // partial slot of the CTA before
   uint32_t b, head;  // sequence; kv head * blocks + block
 };
@@ -86,13 +89,20 @@ struct AttArgs {
   int* err;
 };
 
-__device__ __forceinline__ uint4 ldg_stream(const uint16_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
+// 16 bytes into r if `on`, else r stays: predicated, so that loads stay in one
+// run without branches between them.
+__device__ __forceinline__ void ldg_if(uint4& r, const void* p, bool on) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@p ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
+      : "l"(p), "r"(uint32_t(on)));
 }
+// 16 bytes to shared memory, zeros if not `on`.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <bool BF16>
 __device__ __forceinline__ void mma16(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -134,12 +144,16 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
   return __shfl_sync(0xffffffffu, v, src);
 }
 
-// Where unit u lies. prefix[b] counts the 16-slot tiles of the sequences before b.
+// The line that is shared out: the pairs (sequence, kv head, block) in order,
+// each kPairCost steps and then a step for every unit. prefix[b] counts the
+// steps of one head of the sequences before b; an empty sequence has none.
 struct Place {
-  uint32_t b, head, tile, tiles;
+  uint32_t b, head;  // kv head * blocks + block
+  uint32_t begin;    // the pair's first step
+  uint32_t tiles;    // its units: steps begin + kPairCost ...
 };
-__device__ __forceinline__ Place place_of(uint64_t u, const uint32_t* prefix, uint32_t sequences, uint32_t heads) {
-  const uint64_t t = u / heads;  // tiles of earlier sequences all have `heads` units each
+__device__ __forceinline__ Place place_of(uint32_t u, const uint32_t* prefix, uint32_t sequences, uint32_t heads) {
+  const uint32_t t = u / heads;
   uint32_t lo = 0, hi = sequences;  // prefix[lo] <= t < prefix[hi]
   while (hi - lo > 1) {
     const uint32_t mid = (lo + hi) / 2;
@@ -148,22 +162,31 @@ __device__ __forceinline__ Place place_of(uint64_t u, const uint32_t* prefix, ui
   }
   Place p;
   p.b = lo;
-  p.tiles = prefix[lo + 1] - prefix[lo];
-  const uint64_t in = u - uint64_t(prefix[lo]) * heads;
-  p.head = uint32_t(in / p.tiles);
-  p.tile = uint32_t(in - uint64_t(p.head) * p.tiles);
+  const uint32_t steps = prefix[lo + 1] - prefix[lo], first = prefix[lo] * heads;
+  p.head = (u - first) / steps;
+  p.begin = first + p.head * steps;
+  p.tiles = steps - kPairCost;
   return p;
 }
+__device__ __forceinline__ void next_place(Place& p, const uint32_t* prefix, uint32_t heads) {
+  p.begin += p.tiles + kPairCost;
+  if (++p.head < heads) return;
+  p.head = 0;
+  do ++p.b;
+  while (prefix[p.b + 1] == prefix[p.b]);
+  p.tiles = prefix[p.b + 1] - prefix[p.b] - kPairCost;
+}
 
-// prefix[0..sequences] of the tiles of every sequence, by the whole CTA.
-__device__ __forceinline__ void tile_prefix(const AttArgs& a, uint32_t* prefix, uint32_t* s_warp) {
+// prefix[0..sequences], by the whole CTA.
+__device__ __forceinline__ void step_prefix(const AttArgs& a, uint32_t* prefix, uint32_t* s_warp) {
   const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
   uint32_t run = 0;
   if (threadIdx.x == 0) prefix[0] = 0;
   for (uint32_t base = 0; base < a.kv.sequences; base += blockDim.x) {
     const uint32_t i = base + threadIdx.x;
     uint32_t n = 0;
-    if (i < a.kv.sequences) n = (checked_length(a.lengths[i], a.kv.max_tokens, a.err) + kUnit - 1) / kUnit;
+    if (i < a.kv.sequences) n = checked_length(a.lengths[i], a.kv.max_tokens, a.err);
+    n = n ? (n + kUnit - 1) / kUnit + kPairCost : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t v = __shfl_up_sync(0xffffffffu, n, o);
@@ -181,9 +204,29 @@ __device__ __forceinline__ void tile_prefix(const AttArgs& a, uint32_t* prefix, 
   }
 }
 
-// First unit of share i of n. Units stay below 2^50 (2^32 tiles, 2^18 heads),
-// shares below 2^12.
-__device__ __forceinline__ uint64_t share(uint64_t units, uint32_t i, uint32_t n) { return units * i / n; }
+// Even shares of `steps` for n takers: share i begins at i * steps / n.
+struct Shares {
+  uint32_t each, rest, n;
+  __device__ __forceinline__ Shares(uint32_t steps, uint32_t takers) : each(steps / takers), rest(steps % takers), n(takers) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * each + i * rest / n; }  // i, rest < 2^12
+};
+
+// 8 dims of a query head whose sums are complete: max (base 2), sum, values.
+template <int HD>
+__device__ __forceinline__ void finish(const AttArgs& a, const Place& at, uint32_t head, uint32_t chunk, float m, float l,
+                                       const float* v) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing left: zeros
+  float o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = v[j] * inv;
+  store8(a.out, at.b * a.o_ss + head * a.o_hs + chunk * 8, a.elem, a.o_wide, o);
+  if (chunk == 0) {
+    const float z = l == 0.f ? -INFINITY : m + log2f(l);
+    const uint64_t i = uint64_t(at.b) * a.qh + head;
+    if (a.lse) a.lse[i] = z * kLn2;
+    if (a.lse2) a.lse2[i] = z;
+  }
+}
 
 template <int HD, bool BF16, int TQ, int TP>
 __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_kernel(const __grid_constant__ AttArgs a) {
@@ -195,15 +238,15 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
   extern __shared__ __align__(16) float smem[];
   // per warp: [query terms, later the partial of the last pair][partial of the first pair]
   __shared__ uint32_t s_warp[NW];
-  __shared__ int64_t s_pair[NW][2];
+  __shared__ Place s_part[2 * NW];  // pairs of the warps' partials; tiles 0: no partial
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + NW * kRegion);
   const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5, n8 = lane >> 2, c4 = lane & 3;
   const uint32_t heads = a.kv.kv_heads * a.blocks;
-  if (threadIdx.x < 2 * NW) s_pair[threadIdx.x / 2][threadIdx.x % 2] = -1;
+  if (threadIdx.x < 2 * NW) s_part[threadIdx.x].tiles = 0;
   pdl_launch_dependents();
   pdl_wait();
-  tile_prefix(a, prefix, s_warp);
-  const uint64_t units = uint64_t(prefix[a.kv.sequences]) * heads;
+  step_prefix(a, prefix, s_warp);
+  const uint32_t steps = prefix[a.kv.sequences] * heads;
   // rows of empty sequences
   for (uint32_t b = blockIdx.x; b < a.kv.sequences; b += gridDim.x) {
     if (prefix[b + 1] != prefix[b]) continue;
@@ -215,97 +258,75 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
     if (a.lse)
       for (uint32_t h = threadIdx.x; h < a.qh; h += NW * 32) a.lse[uint64_t(b) * a.qh + h] = -INFINITY;
   }
-  // few units: as many CTAs as give every warp one
-  const uint32_t ctas = uint32_t(min(uint64_t(gridDim.x), (units + NW - 1) / NW));
-  const uint32_t cta = blockIdx.x;
-  if (threadIdx.x == 0) {
+  // little work: fewer CTAs, so that most warps still have a unit
+  const uint32_t ctas = min(gridDim.x, (steps + NW - 1) / NW), cta = blockIdx.x;
+  if (cta >= ctas) {
+    if (threadIdx.x == 0) a.join[cta].last = -1;
+    return;
+  }
+  const Shares cta_share(steps, ctas), warp_share(steps, ctas * NW);
+  const uint32_t cu0 = cta_share.begin(cta), cu1 = cta_share.begin(cta + 1);
+  if (threadIdx.x == NW * 32 - 1) {
     Join j = {-1, 0, 0, 0};
-    if (cta > 0 && cta < ctas) {
-      const uint64_t cu = share(units, cta, ctas), before = share(units, cta - 1, ctas);
-      const Place p = place_of(cu, prefix, a.kv.sequences, heads);
-      const uint64_t first = cu - p.tile, end = first + p.tiles;
-      if (first < cu && first >= before) {  // the first border inside this pair
-        j.last = int32_t((end * ctas + units - 1) / units - 1);  // whose share holds unit end - 1
-        j.slot0 = first == before ? 0 : 1;
+    if (cta > 0) {
+      const Place p = place_of(cu0, prefix, a.kv.sequences, heads);
+      const uint32_t first = p.begin + kPairCost, end = first + p.tiles, before = cta_share.begin(cta - 1);
+      if (first < cu0 && (before <= first)) {  // the first border among this pair's units
+        j.slot0 = p.begin <= before ? 0 : 1;
+        uint32_t last = cta;
+        for (uint32_t step = 128; step; step >>= 1)  // whose share holds step end - 1
+          if (last + step < ctas && cta_share.begin(last + step) < end) last += step;
+        j.last = int32_t(last);
         j.b = p.b;
         j.head = p.head;
       }
     }
     a.join[cta] = j;
   }
-  if (cta >= ctas) return;
-  const uint64_t u0 = share(units, cta * NW + w, ctas * NW), u1 = share(units, cta * NW + w + 1, ctas * NW);
+  const uint32_t u0 = warp_share.begin(cta * NW + w), u1 = warp_share.begin(cta * NW + w + 1);
   float* region = smem + w * kRegion;
-  uint4* s_q = reinterpret_cast<uint4*>(region) + lane;  // [term][step][lane]: a lane reads what it wrote
+  uint4* s_q = reinterpret_cast<uint4*>(region) + lane;  // [step][term][lane]: a lane reads what it wrote
   const uint32_t chunks = a.kv.hd / 8;
 
-  uint64_t u = u0;
-  while (u < u1) {
-    const Place at = place_of(u, prefix, a.kv.sequences, heads);
+  Place at;
+  if (u0 < u1) at = place_of(u0, prefix, a.kv.sequences, heads);
+  uint4 kr[2][KK] = {}, vr[4][KV] = {};  // places that no load fills (dims past head_dim) stay zero
+  for (uint32_t u = u0; u < u1; u = at.begin + at.tiles + kPairCost, u < u1 ? next_place(at, prefix, heads) : void()) {
+    const uint32_t first = at.begin + kPairCost;
+    const uint32_t t_begin = u > first ? u - first : 0, t_end = min(u1, first + at.tiles) - first;
+    if (u1 <= first || t_begin >= t_end) continue;  // the share ends before the pair's units
     const uint32_t kvh = at.head / a.blocks, col0 = (at.head - kvh * a.blocks) * kCols;
     const uint32_t cols = min(kCols, a.group - col0), qhead0 = kvh * a.group + col0;
-    const uint32_t t_end = uint32_t(min(uint64_t(at.tiles), at.tile + (u1 - u)));
-    const uint32_t len = checked_length(a.lengths[at.b], a.kv.max_tokens, a.err);
     const int32_t* row = a.kv.pages + at.b * a.kv.pages_stride;
 
-    // queries into 16-bit terms; columns past the group are zero
-    float col_scale = a.scale;
-    {
-      float q[KK][8];
-      float big = 0.f;
-#pragma unroll
-      for (int s = 0; s < KK; ++s) {
-        const uint32_t ch = 4 * s + c4;
-        if (n8 < cols && ch < chunks) {
-          load8(a.q, at.b * a.q_ss + (qhead0 + n8) * a.q_hs + ch * 8, a.elem, a.q_wide, q[s]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) q[s][j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(q[s][j]));
-      }
-      if constexpr (!BF16) {  // to a maximum in [2^14, 2^15): small elements beside large ones keep their bits
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        int e = 0;
-        if (big > 0.f && big < INFINITY) e = max(-100, ilogbf(big)) - 14;
-        const float down = ldexpf(1.f, -e);
-        col_scale *= ldexpf(1.f, e);
-#pragma unroll
-        for (int s = 0; s < KK; ++s)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) q[s][j] *= down;
-      }
-#pragma unroll
-      for (int s = 0; s < KK; ++s)
-#pragma unroll
-        for (int t = 0; t < TQ; ++t) {
-          uint4 r;
-          r.x = take_term<BF16>(q[s][0], q[s][1]);
-          r.y = take_term<BF16>(q[s][2], q[s][3]);
-          r.z = take_term<BF16>(q[s][4], q[s][5]);
-          r.w = take_term<BF16>(q[s][6], q[s][7]);
-          s_q[(t * KK + s) * 32] = r;
-        }
-    }
-    // scale of the lane's two columns of S^T
-    const float sc0 = __shfl_sync(0xffffffffu, col_scale, c4 * 8), sc1 = __shfl_sync(0xffffffffu, col_scale, c4 * 8 + 4);
-
-    float acc[KV * 4][4] = {};
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    uint4 kr[2][KK], vr[4][KV];
-
-    // The page of slot (unit, lane % 16), asked for two units ahead of its use;
-    // a negative number stands for "no slot".
+    // The page of slot (unit, lane % 16), asked for two units ahead of its use.
     auto page_of = [&](uint32_t tile) -> int32_t {
       const uint32_t t = tile * kUnit + (lane & 15);
-      return tile < t_end && t < len ? __ldg(row + div_of(t, a.kv.page)) : -1;
+      return tile < t_end && t < a.kv.max_tokens ? __ldg(row + div_of(t, a.kv.page)) : -1;
     };
+    int32_t page_next = page_of(t_begin + 1);
+    const int32_t page_first = page_of(t_begin);
+    const uint32_t len = checked_length(a.lengths[at.b], a.kv.max_tokens, a.err);
+    // Queries as they are, each lane's own into its places of shared memory;
+    // rolled loops here and at the pair's end: code that runs once a pair costs
+    // its instruction fetches.
+    const uint64_t q0 = at.b * a.q_ss + uint64_t(qhead0 + n8) * a.q_hs;
+    if (a.q_wide) {
+      const uint8_t* from = static_cast<const uint8_t*>(a.q) + q0 * elem_bytes(a.elem);
+#pragma unroll 1
+      for (uint32_t s = 0; s < KK; ++s) {
+        const uint32_t ch = 4 * s + c4;
+        const bool on = n8 < cols && ch < chunks;
+        const uint8_t* x = on ? from + ch * 8 * elem_bytes(a.elem) : static_cast<const uint8_t*>(a.q);
+        cp_async16(s_q + s * TQ * 32, x, on);
+        if (TQ > 1 && a.elem == SI_ELEM_F32) cp_async16(s_q + (s * TQ + 1) * 32, on ? x + 16 : x, on);
+      }
+    }
     auto cell_of = [&](uint32_t tile, int32_t page) -> uint64_t {
       const uint32_t t = tile * kUnit + (lane & 15);
-      const uint64_t cell = paged_cell(a.kv, page, t - div_of(t, a.kv.page) * a.kv.page.d, kvh);
-      if (cell == kNoCell && tile < t_end && t < len) atomicOr(a.err, KERR_BAD_INDEX);
+      const bool on = tile < t_end && t < len;
+      const uint64_t cell = on ? paged_cell(a.kv, page, t - div_of(t, a.kv.page) * a.kv.page.d, kvh) : kNoCell;
+      if (on && cell == kNoCell) atomicOr(a.err, KERR_BAD_INDEX);
       return cell;
     };
     auto load_k = [&](uint64_t cell, bool& lo, bool& hi) {
@@ -315,41 +336,112 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
 #pragma unroll
       for (int s = 0; s < KK; ++s) {
         const uint32_t ch = 4 * s + c4;
-        kr[0][s] = lo && ch < chunks ? ldg_stream(a.kv.k + c0 + ch * 8) : make_uint4(0, 0, 0, 0);
-        kr[1][s] = hi && ch < chunks ? ldg_stream(a.kv.k + c1 + ch * 8) : make_uint4(0, 0, 0, 0);
+        ldg_if(kr[0][s], a.kv.k + c0 + ch * 8, lo && ch < chunks);
+        ldg_if(kr[1][s], a.kv.k + c1 + ch * 8, hi && ch < chunks);
       }
     };
     auto load_v = [&](uint64_t cell) {
+      // slots that do not exist meet probability 0, and need a finite value
+      if (__any_sync(0xffffffffu, cell == kNoCell)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < KV; ++d) vr[i][d] = make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t c = shfl64(cell, 2 * c4 + (i & 1) + (i >> 1) * 8);
 #pragma unroll
         for (int d = 0; d < KV; ++d) {
           const uint32_t ch = 8 * d + n8;
-          vr[i][d] = c != kNoCell && ch < chunks ? ldg_stream(a.kv.v + c + ch * 8) : make_uint4(0, 0, 0, 0);
+          ldg_if(vr[i][d], a.kv.v + c + ch * 8, c != kNoCell && ch < chunks);
         }
       }
     };
-
     bool lo, hi;
-    uint64_t cell = cell_of(at.tile, page_of(at.tile));
-    int32_t page_next = page_of(at.tile + 1);
+    uint64_t cell = cell_of(t_begin, page_first);
     load_k(cell, lo, hi);
     load_v(cell);
-    for (uint32_t tile = at.tile; tile < t_end; ++tile) {
+    // queries into 16-bit terms, in place; columns past the group are zero
+    auto raw = [&](uint32_t s, float x[8]) {
+      const uint32_t ch = 4 * s + c4;
+      if (a.q_wide) {
+        const uint4 r = s_q[s * TQ * 32];
+        if (TQ > 1 && a.elem == SI_ELEM_F32) {
+          const uint4 z = s_q[(s * TQ + 1) * 32];
+          x[0] = as_f(r.x), x[1] = as_f(r.y), x[2] = as_f(r.z), x[3] = as_f(r.w);
+          x[4] = as_f(z.x), x[5] = as_f(z.y), x[6] = as_f(z.z), x[7] = as_f(z.w);
+        } else {
+          const uint32_t h[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = elem_to_f(uint16_t(h[j / 2] >> (j % 2 * 16)), a.elem);
+        }
+      } else if (n8 < cols && ch < chunks) {
+        load8(a.q, q0 + ch * 8, a.elem, false, x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      }
+    };
+    cp_async_wait();
+    float col_scale = a.scale, down = 1.f;
+    if constexpr (!BF16) {  // to a maximum in [2^14, 2^15): small elements beside large ones keep their bits
+      float big = 0.f;
+#pragma unroll 1
+      for (uint32_t s = 0; s < KK; ++s) {
+        float x[8];
+        raw(s, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[j]));
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      int e = 0;
+      if (big > 0.f && big < INFINITY) e = max(-100, ilogbf(big)) - 14;
+      down = ldexpf(1.f, -e);
+      col_scale *= ldexpf(1.f, e);
+    }
+#pragma unroll 1
+    for (uint32_t s = 0; s < KK; ++s) {
+      float x[8];
+      raw(s, x);
+      if constexpr (!BF16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= down;
+      }
+#pragma unroll
+      for (int t = 0; t < TQ; ++t) {
+        uint4 r;
+        r.x = take_term<BF16>(x[0], x[1]);
+        r.y = take_term<BF16>(x[2], x[3]);
+        r.z = take_term<BF16>(x[4], x[5]);
+        r.w = take_term<BF16>(x[6], x[7]);
+        s_q[(s * TQ + t) * 32] = r;
+      }
+    }
+    // scale of the lane's two columns of S^T
+    const float sc0 = __shfl_sync(0xffffffffu, col_scale, c4 * 8), sc1 = __shfl_sync(0xffffffffu, col_scale, c4 * 8 + 4);
+
+    float acc[KV * 4][4] = {};
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    for (uint32_t tile = t_begin; tile < t_end; ++tile) {
       const int32_t page_after = page_of(tile + 2);
-      float s[4] = {};
+      // The leading terms in two chains, the small ones in a third: shorter
+      // chains of dependent products, and fewer roundings of a large sum.
+      float s[4] = {}, s_odd[4] = {}, s_low[4] = {};
 #pragma unroll
       for (int st = 0; st < KK; ++st) {
         const uint4 x = kr[0][st], y = kr[1][st];
         const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
 #pragma unroll
-        for (int t = TQ - 1; t >= 0; --t) {  // small terms first
-          const uint4 qv = s_q[(t * KK + st) * 32];
-          mma16<BF16>(s, a0, qv.x, qv.y);
-          mma16<BF16>(s, a1, qv.z, qv.w);
+        for (int t = 0; t < TQ; ++t) {
+          const uint4 qv = s_q[(st * TQ + t) * 32];
+          mma16<BF16>(t ? s_low : s, a0, qv.x, qv.y);
+          mma16<BF16>(t ? s_low : s_odd, a1, qv.z, qv.w);
         }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += s_odd[i] + (TQ > 1 ? s_low[i] : 0.f);
       const bool lo_now = lo, hi_now = hi;
       cell = cell_of(tile + 1, page_next);
       page_next = page_after;
@@ -408,8 +500,18 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
         for (int j = 0; j < 4; ++j) {
           const uint32_t av[4] = {__byte_perm(v0[j], v1[j], 0x5410), __byte_perm(v0[j], v1[j], 0x7632),
                                   __byte_perm(v2[j], v3[j], 0x5410), __byte_perm(v2[j], v3[j], 0x7632)};
+          if constexpr (TQ > 1) {
+            // The tensor core cuts its sums off: the unit's products are summed
+            // by themselves and added, rounded, to the running sum.
+            float o[4] = {};
 #pragma unroll
-          for (int t = TP - 1; t >= 0; --t) mma16<BF16>(acc[d * 4 + j], av, pb[t][0], pb[t][1]);
+            for (int t = TP - 1; t >= 0; --t) mma16<BF16>(o, av, pb[t][0], pb[t][1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[d * 4 + j][i] += o[i];
+          } else {
+#pragma unroll
+            for (int t = TP - 1; t >= 0; --t) mma16<BF16>(acc[d * 4 + j], av, pb[t][0], pb[t][1]);
+          }
         }
       }
       load_v(cell);
@@ -420,161 +522,152 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
       l0 += __shfl_xor_sync(0xffffffffu, l0, o);
       l1 += __shfl_xor_sync(0xffffffffu, l1, o);
     }
-    if (at.tile == 0 && t_end == at.tiles) {  // a whole pair
+    // The first pair's partial lies beside the queries; another one's lies over
+    // them, as does a whole pair on its way out.
+    const bool whole = t_begin == 0 && t_end == at.tiles;
+    const uint32_t slot = u == u0 && !whole ? 0 : 1;
+    float* part = slot ? region : region + (kRegion - kPart);
+    __syncwarp();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t col = 2 * c4 + c;
-        if (col >= cols) continue;
-        const float l = c ? l1 : l0, inv = l > 0.f ? 1.f / l : 0.f;
+    for (int c = 0; c < 2; ++c) {
+      const uint32_t col = 2 * c4 + c;
 #pragma unroll
-        for (int d = 0; d < KV; ++d) {
-          const uint32_t ch = 8 * d + n8;
-          if (ch >= chunks) continue;
-          float o[8];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            o[2 * j] = acc[d * 4 + j][c] * inv;
-            o[2 * j + 1] = acc[d * 4 + j][2 + c] * inv;
-          }
-          store8(a.out, at.b * a.o_ss + (qhead0 + col) * a.o_hs + ch * 8, a.elem, a.o_wide, o);
-        }
-        if (n8 == 0) {
-          const float z = l > 0.f ? (c ? m1 : m0) - kShift + log2f(l) : -INFINITY;
-          const uint64_t i = uint64_t(at.b) * a.qh + qhead0 + col;
-          if (a.lse) a.lse[i] = z * kLn2;
-          if (a.lse2) a.lse2[i] = z;
-        }
+      for (int d = 0; d < KV; ++d) {
+        float* to = part + col * HD + (8 * d + n8) * 8;
+        *reinterpret_cast<float4*>(to) =
+            make_float4(acc[d * 4][c], acc[d * 4][2 + c], acc[d * 4 + 1][c], acc[d * 4 + 1][2 + c]);
+        *reinterpret_cast<float4*>(to + 4) =
+            make_float4(acc[d * 4 + 2][c], acc[d * 4 + 2][2 + c], acc[d * 4 + 3][c], acc[d * 4 + 3][2 + c]);
       }
-    } else {
-      // the share's first pair beside the queries, another one over them
-      const uint32_t slot = u == u0 ? 0 : 1;
-      float* part = slot ? region : region + (kRegion - kPart);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t col = 2 * c4 + c;
-#pragma unroll
-        for (int d = 0; d < KV; ++d) {
-          float* to = part + col * HD + (8 * d + n8) * 8;
-          *reinterpret_cast<float4*>(to) =
-              make_float4(acc[d * 4][c], acc[d * 4][2 + c], acc[d * 4 + 1][c], acc[d * 4 + 1][2 + c]);
-          *reinterpret_cast<float4*>(to + 4) =
-              make_float4(acc[d * 4 + 2][c], acc[d * 4 + 2][2 + c], acc[d * 4 + 3][c], acc[d * 4 + 3][2 + c]);
-        }
-        if (n8 == 0) {
-          part[kCols * HD + 2 * col] = c ? m1 : m0;
-          part[kCols * HD + 2 * col + 1] = c ? l1 : l0;
-        }
-      }
-      if (lane == 0) s_pair[w][slot] = int64_t(u - at.tile);  // the pair's first unit names it
+      if (n8 == 0) *reinterpret_cast<float2*>(part + kCols * HD + 2 * col) = make_float2(c ? m1 : m0, c ? l1 : l0);
     }
-    u += t_end - at.tile;
-  }
-  __syncthreads();
-  // join the warps' partials, in the order of their units
-  const uint64_t cu0 = share(units, cta, ctas), cu1 = share(units, cta + 1, ctas);
-  for (uint32_t e = 0; e < 2 * NW;) {
-    const int64_t pair = s_pair[e / 2][e % 2];
-    if (pair < 0) {
-      ++e;
+    if (!whole) {
+      if (lane == 0) s_part[2 * w + slot] = at;
       continue;
     }
-    uint32_t stop = e + 1;
-    while (stop < 2 * NW && (s_pair[stop / 2][stop % 2] < 0 || s_pair[stop / 2][stop % 2] == pair)) ++stop;
-    const Place at = place_of(uint64_t(pair), prefix, a.kv.sequences, heads);
+    __syncwarp();
+#pragma unroll 1
+    for (uint32_t i = lane; i < cols * chunks; i += 32) {
+      const uint32_t col = i / chunks, ch = i - col * chunks;
+      const float2 ml = *reinterpret_cast<const float2*>(part + kCols * HD + 2 * col);
+      finish<HD>(a, at, qhead0 + col, ch, ml.x - kShift, ml.y, part + col * HD + ch * 8);
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  // Join the warps' partials in the order of their units: partial e leads its
+  // pair if the one before it is of another pair, and the lead's outputs are
+  // shared out over all threads together with those of the other leads.
+  constexpr uint32_t kItems = kCols * (HD / 8);
+  for (uint32_t i = threadIdx.x; i < 2 * NW * kItems; i += NW * 32) {
+    const uint32_t e = i / kItems, col = i % kItems / (HD / 8), ch = i % (HD / 8);
+    const Place at = s_part[e];
+    if (at.tiles == 0) continue;
+    uint32_t before = e;  // the nearest partial before e
+    while (before > 0 && s_part[before - 1].tiles == 0) --before;
+    if (before > 0 && s_part[before - 1].begin == at.begin) continue;
     const uint32_t kvh = at.head / a.blocks, col0 = (at.head - kvh * a.blocks) * kCols;
     const uint32_t cols = min(kCols, a.group - col0), qhead0 = kvh * a.group + col0;
-    const bool whole = uint64_t(pair) >= cu0 && uint64_t(pair) + at.tiles <= cu1;
-    float* part = a.part + (uint64_t(cta) * 2 + (uint64_t(pair) <= cu0 ? 0 : 1)) * kPart;
-    for (uint32_t i = threadIdx.x; i < cols * (HD / 8); i += NW * 32) {
-      const uint32_t col = i / (HD / 8), ch = i - col * (HD / 8);
-      float m = -INFINITY;
-      for (uint32_t x = e; x < stop; ++x)
-        if (s_pair[x / 2][x % 2] >= 0)
-          m = fmaxf(m, (smem + (x / 2) * kRegion + (x % 2 ? 0 : kRegion - kPart))[kCols * HD + 2 * col]);
-      float l = 0.f, o[8] = {};
-      for (uint32_t x = e; x < stop; ++x) {
-        if (s_pair[x / 2][x % 2] < 0) continue;
-        const float* from = smem + (x / 2) * kRegion + (x % 2 ? 0 : kRegion - kPart);
-        const float mx = from[kCols * HD + 2 * col];
-        if (mx == -INFINITY) continue;
-        const float f = exp2f(mx - m);
-        l += f * from[kCols * HD + 2 * col + 1];
-        const float4 v0 = *reinterpret_cast<const float4*>(from + col * HD + ch * 8);
-        const float4 v1 = *reinterpret_cast<const float4*>(from + col * HD + ch * 8 + 4);
-        o[0] += f * v0.x, o[1] += f * v0.y, o[2] += f * v0.z, o[3] += f * v0.w;
-        o[4] += f * v1.x, o[5] += f * v1.y, o[6] += f * v1.z, o[7] += f * v1.w;
-      }
-      if (whole) {
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (col >= cols) continue;
+    float m = -INFINITY, l = 0.f, o[8] = {};
+    for (uint32_t x = e; x < 2 * NW; ++x) {
+      if (s_part[x].tiles == 0) continue;
+      if (s_part[x].begin != at.begin) break;
+      const float* from = smem + (x / 2) * kRegion + (x % 2 ? 0 : kRegion - kPart);
+      const float2 ml = *reinterpret_cast<const float2*>(from + kCols * HD + 2 * col);
+      if (ml.x == -INFINITY) continue;
+      const float g = fmaxf(m, ml.x), f0 = exp2f(m - g), f1 = exp2f(ml.x - g);
+      m = g;
+      l = l * f0 + ml.y * f1;
+      const float4 v0 = *reinterpret_cast<const float4*>(from + col * HD + ch * 8);
+      const float4 v1 = *reinterpret_cast<const float4*>(from + col * HD + ch * 8 + 4);
+      const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] *= inv;
-        if (ch < chunks) store8(a.out, at.b * a.o_ss + (qhead0 + col) * a.o_hs + ch * 8, a.elem, a.o_wide, o);
-        if (ch == 0) {
-          const float z = l > 0.f ? m - kShift + log2f(l) : -INFINITY;
-          const uint64_t y = uint64_t(at.b) * a.qh + qhead0 + col;
-          if (a.lse) a.lse[y] = z * kLn2;
-          if (a.lse2) a.lse2[y] = z;
-        }
-      } else {
-        *reinterpret_cast<float4*>(part + col * HD + ch * 8) = make_float4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<float4*>(part + col * HD + ch * 8 + 4) = make_float4(o[4], o[5], o[6], o[7]);
-        if (ch == 0) {
-          part[kCols * HD + 2 * col] = m;
-          part[kCols * HD + 2 * col + 1] = l;
-        }
+      for (int j = 0; j < 8; ++j) o[j] = o[j] * f0 + v[j] * f1;
+    }
+    const uint32_t first = at.begin + kPairCost;
+    if (first >= cu0 && first + at.tiles <= cu1) {
+      if (ch < chunks) finish<HD>(a, at, qhead0 + col, ch, m - kShift, l, o);
+    } else {
+      float* part = a.part + (uint64_t(cta) * 2 + (at.begin <= cu0 ? 0 : 1)) * kPart;
+      *reinterpret_cast<float4*>(part + col * HD + ch * 8) = make_float4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<float4*>(part + col * HD + ch * 8 + 4) = make_float4(o[4], o[5], o[6], o[7]);
+      if (ch == 0) {
+        part[kCols * HD + 2 * col] = m;
+        part[kCols * HD + 2 * col + 1] = l;
       }
     }
-    e = stop;
   }
 }
 
 // Joins the partials of the pairs that cross CTA borders. Block (i, column):
-// the pair whose first border is the one before CTA i, one query head of it.
+// the pair whose first border is the one before CTA i + 1, one query head of
+// it. A pair may lie in as many partials as there are CTAs; four groups of
+// threads take every fourth each, in batches whose loads are all in flight.
+constexpr int kJoinGroups = 4, kJoinBatch = 10;
 template <int HD>
-__global__ void __launch_bounds__(HD) paged_join_kernel(const __grid_constant__ AttArgs a, float shift) {
+__global__ void __launch_bounds__(HD * kJoinGroups) paged_join_kernel(const __grid_constant__ AttArgs a, float shift) {
   constexpr uint32_t kPart = kCols * (HD + 2);
+  __shared__ float s_o[kJoinGroups][HD], s_m[kJoinGroups], s_l[kJoinGroups];
   pdl_launch_dependents();
   pdl_wait();
   const Join j = a.join[blockIdx.x + 1];
   if (j.last < 0) return;
   const uint32_t kvh = j.head / a.blocks, col0 = (j.head - kvh * a.blocks) * kCols, col = blockIdx.y;
   if (col >= min(kCols, a.group - col0)) return;
-  const uint32_t first = blockIdx.x, d = threadIdx.x;  // CTA before the border
-  auto part = [&](uint32_t c) { return a.part + (uint64_t(c) * 2 + (c == first ? j.slot0 : 0)) * kPart; };
+  const uint32_t first = blockIdx.x, d = threadIdx.x % HD, grp = threadIdx.x / HD;  // first: the CTA before the border
   float m = -INFINITY, l = 0.f, o = 0.f;
-  for (uint32_t c = first; c <= uint32_t(j.last); c += 8) {
-    float mx[8], lx[8], vx[8];
+  for (uint32_t c = first + grp; c <= uint32_t(j.last); c += kJoinGroups * kJoinBatch) {
+    float mx[kJoinBatch], lx[kJoinBatch], vx[kJoinBatch];
+#pragma unroll
+    for (int i = 0; i < kJoinBatch; ++i) {
+      const uint32_t x = c + i * kJoinGroups;
+      mx[i] = -INFINITY, lx[i] = 0.f, vx[i] = 0.f;
+      if (x <= uint32_t(j.last)) {
+        const float* p = a.part + (uint64_t(x) * 2 + (x == first ? j.slot0 : 0)) * kPart;
+        const float2 ml = *reinterpret_cast<const float2*>(p + kCols * HD + 2 * col);
+        mx[i] = ml.x;
+        lx[i] = ml.y;
+        vx[i] = p[col * HD + d];
+      }
+    }
     float g = m;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool in = c + i <= uint32_t(j.last);
-      const float* p = part(in ? c + i : first);
-      mx[i] = in ? p[kCols * HD + 2 * col] : -INFINITY;
-      lx[i] = p[kCols * HD + 2 * col + 1];
-      vx[i] = p[col * HD + d];
-      g = fmaxf(g, mx[i]);
-    }
+    for (int i = 0; i < kJoinBatch; ++i) g = fmaxf(g, mx[i]);
     if (g == -INFINITY) continue;
     const float f = exp2f(m - g);
     l *= f;
     o *= f;
     m = g;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float f = mx[i] == -INFINITY ? 0.f : exp2f(mx[i] - g);
+    for (int i = 0; i < kJoinBatch; ++i) {
+      const float f = exp2f(mx[i] - g);
       l += f * lx[i];
       o += f * vx[i];
     }
   }
+  s_o[grp][d] = o;
+  if (d == 0) s_m[grp] = m, s_l[grp] = l;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int i = 1; i < kJoinGroups; ++i) {
+    const float mi = s_m[i];
+    if (mi == -INFINITY) continue;
+    const float g = fmaxf(m, mi), f0 = exp2f(m - g), f1 = exp2f(mi - g);
+    m = g;
+    l = l * f0 + s_l[i] * f1;
+    o = o * f0 + s_o[i][d] * f1;
+  }
   const uint32_t head = kvh * a.group + col0 + col;
   if (d < a.kv.hd) {
     const uint64_t at = j.b * a.o_ss + head * a.o_hs + d;
-    const float v = l > 0.f ? o / l : 0.f;
+    const float v = l == 0.f ? 0.f : o / l;
     if (a.elem == SI_ELEM_F32) static_cast<float*>(a.out)[at] = v;
     else static_cast<uint16_t*>(a.out)[at] = f_to_elem(v, a.elem);
   }
   if (d == 0) {
-    const float z = l > 0.f ? m - shift + log2f(l) : -INFINITY;
+    const float z = l == 0.f ? -INFINITY : m - shift + log2f(l);
     const uint64_t y = uint64_t(j.b) * a.qh + head;
     if (a.lse) a.lse[y] = z * kLn2;
     if (a.lse2) a.lse2[y] = z;
@@ -621,11 +714,23 @@ uint64_t work_bytes(const si_paged_kv& kv, uint32_t qh, bool weights) {
   return n;
 }
 
+// Steps of the line that is shared out, if every sequence fills its pages.
+uint64_t most_steps(const si_paged_kv& kv, uint32_t qh) {
+  const uint64_t blocks = (qh / kv.kv_heads + kCols - 1) / kCols;
+  const uint64_t tiles = (uint64_t(kv.max_pages) * kv.page_tokens + kUnit - 1) / kUnit + kPairCost;
+  const unsigned __int128 n = (unsigned __int128)tiles * kv.sequences * kv.kv_heads * blocks;
+  return n >> 64 ? ~uint64_t(0) : uint64_t(n);
+}
+
 int check_heads(const si_paged_kv* kv, uint32_t qh, std::string* msg) {
   if (int rc = check_paged_kv(kv, msg)) return rc;
   if (qh == 0 || qh % kv->kv_heads || qh > 65535) {
     *msg = "paged attention query heads must be a multiple of the kv heads";
     return SI_E_INVALID;
+  }
+  if (most_steps(*kv, qh) > 0xffffffffull) {
+    *msg = "paged attention takes page tables of less than 2^32 units of 16 slots, over all sequences and heads";
+    return SI_E_UNSUPPORTED;
   }
   return SI_OK;
 }
@@ -665,7 +770,7 @@ cudaError_t launch(const AttArgs& p, uint32_t grid, cudaStream_t s) {
   PdlLaunch l(dim3(grid), dim3(Shape<HD>::kWarps * 32), smem, s);
   if (cudaError_t e = cudaLaunchKernelEx(&l.cfg, kernel, p)) return e;
   if (grid == 1) return cudaSuccess;
-  PdlLaunch j(dim3(grid - 1, std::min(kCols, p.group)), dim3(HD), 0, s);
+  PdlLaunch j(dim3(grid - 1, std::min(kCols, p.group)), dim3(HD * kJoinGroups), 0, s);
   return cudaLaunchKernelEx(&j.cfg, paged_join_kernel<HD>, p, BF16 ? 0.f : 15.f);
 }
 
@@ -722,7 +827,7 @@ extern "C" int si_paged_attention_dev(si_ctx* ctx, const si_paged_kv* kv, const 
     p.scores = reinterpret_cast<float*>(more + round16(uint64_t(kv->sequences) * p.qh * 4));
   }
   const cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-  const uint64_t most = uint64_t(kv->sequences) * ((p.kv.max_tokens + kUnit - 1) / kUnit) * kv->kv_heads * p.blocks;
+  const uint64_t most = most_steps(*kv, p.qh);
   const uint32_t nw = warps_of(kv->head_dim);
   const uint32_t grid = uint32_t(std::min<uint64_t>(std::min<uint32_t>(ctx->sm_count, kMaxCtas), (most + nw - 1) / nw));
   const bool bf16 = kv->elem == SI_ELEM_BF16;

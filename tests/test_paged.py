@@ -167,7 +167,7 @@ KV_FAULTS = [("elem", 0, UNSUPPORTED), ("elem", 3, UNSUPPORTED), ("kv_heads", 0,
              ("head_dim", 0, INVALID), ("head_dim", 12, UNSUPPORTED), ("head_dim", 264, UNSUPPORTED),
              ("page_tokens", 0, INVALID), ("page_tokens", 1 << 30, UNSUPPORTED), ("num_pages", 0, INVALID),
              ("num_pages", 1 << 31, UNSUPPORTED), ("max_pages", 0, INVALID), ("sequences", 0, INVALID),
-             ("sequences", 8193, UNSUPPORTED), ("pages_stride", 1, INVALID), ("page_stride", 9, INVALID),
+             ("sequences", 4097, UNSUPPORTED), ("pages_stride", 1, INVALID), ("page_stride", 9, INVALID),
              ("head_stride", 4, INVALID), ("token_stride", 12, INVALID), ("page_stride", 1 << 62, INVALID),
              ("k", None, INVALID), ("v", None, INVALID), ("pages", None, INVALID)]
 
