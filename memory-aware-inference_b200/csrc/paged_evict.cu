@@ -9,13 +9,14 @@
 // below the new length and the kept slots behind it; pair i moves from the
 // i-th kept slot to the i-th hole.
 //
-// Selection: a cluster of 1 to 8 CTAs a (sequence, kv head); every key is read
-// from global memory once and stays in shared memory for the three digits and
-// the walk; histograms and counts meet over distributed shared memory. Moves: a second
-// kernel over all pairs of all heads, because a cut of a long prompt
-// moves megabytes where the selection is a few small scans; 16 bytes a thread
-// and access. The selection is bound by latency (about five cluster barriers), the
-// moves by bandwidth.
+// Selection: one CTA a (sequence, kv head), or a cluster of up to 8 for long
+// sequences; every key is read from global memory once and stays in shared
+// memory for the three digits and the walk; histograms and counts meet over
+// distributed shared memory. Small CTAs where the keys are few: the time is that of a
+// chain of small scans, so as many rows as possible run beside each other.
+// Moves: a second kernel over all pairs of all heads, because a cut of a long
+// prompt moves megabytes where the selection is a few scans. Selection is bound by
+// latency, moves by bandwidth.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -25,7 +26,6 @@
 namespace si {
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
 constexpr uint32_t kBins = 2048;
 constexpr uint32_t kCtaSlots = 49152;  // keys in a CTA's shared memory
 constexpr uint32_t kMaxCluster = 8;
@@ -44,7 +44,7 @@ struct EvictArgs {
   uint32_t budget, sink, recent;
   uint32_t most;  // longest length that the page table and the weights' rows have room for
   uint32_t room;  // entries of a move list
-  uint2* moves;      // [sequence * kv_heads + head][room] (from, to)
+  uint32_t* moves;   // [sequence * kv_heads + head][2][room]: from, to
   uint32_t* counts;  // [sequence * kv_heads + head]
   int* err;
 };
@@ -66,17 +66,41 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+template <bool CLUSTER>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (CLUSTER)
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else
+    __syncthreads();
+}
+__device__ __forceinline__ uint32_t peer_address(const uint32_t* p, uint32_t rank) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  return at;
 }
 __device__ __forceinline__ uint32_t peer_u32(const uint32_t* p, uint32_t rank) {
-  uint32_t at, v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_address(p, rank)) : "memory");
   return v;
+}
+// N neighbouring words of another CTA, zeros if not `on`.
+template <uint32_t N>
+__device__ __forceinline__ void peer_bins(uint32_t* v, const uint32_t* p, uint32_t rank, bool on) {
+  static_assert(N == 2 || N == 4, "bins of a thread");
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) v[i] = 0;
+  if (!on) return;
+  if constexpr (N == 2)
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(peer_address(p, rank)) : "memory");
+  else
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(peer_address(p, rank))
+                 : "memory");
 }
 
 // Exclusive prefix of one value a thread over the CTA; *total gets the sum.
+template <int THREADS>
 __device__ __forceinline__ uint32_t cta_prefix(uint32_t v, uint32_t* s_w, uint32_t* total) {
   const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   uint32_t x = v;
@@ -88,7 +112,7 @@ __device__ __forceinline__ uint32_t cta_prefix(uint32_t v, uint32_t* s_w, uint32
   __syncthreads();
   if (lane == 31) s_w[w] = x;
   __syncthreads();
-  uint32_t y = s_w[lane];  // kWarps == 32
+  uint32_t y = lane < THREADS / 32 ? s_w[lane] : 0;
   const uint32_t mine = y;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -99,10 +123,13 @@ __device__ __forceinline__ uint32_t cta_prefix(uint32_t v, uint32_t* s_w, uint32
   return __shfl_sync(0xffffffffu, y - mine, w) + x - v;
 }
 
-__global__ void __launch_bounds__(kThreads, 1) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+template <int THREADS, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+  constexpr uint32_t kWarps = THREADS / 32, kMine = kBins / THREADS;  // bins of a thread
   extern __shared__ uint32_t s_key[];
-  __shared__ uint32_t s_bin[kBins], s_w[32], s_found[2], s_ties, s_moves[2];
-  const uint32_t rank = cluster_rank(), size = cluster_size();
+  __shared__ __align__(16) uint32_t s_bin[kBins];
+  __shared__ uint32_t s_w[32], s_found[3], s_ties, s_moves[2];
+  const uint32_t rank = CLUSTER ? cluster_rank() : 0, size = CLUSTER ? cluster_size() : 1;
   const uint32_t row = blockIdx.x / size, b = row / a.kv.kv_heads;
   const uint32_t tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   pdl_launch_dependents();
@@ -115,86 +142,139 @@ __global__ void __launch_bounds__(kThreads, 1) evict_select_kernel(const __grid_
     // the new length is written by the second kernel
     if (a.len_out != a.len_in) a.len_out[b] = int32_t(m);
   }
-  // a CTA's slots, a multiple of 1024 so that every warp has whole rows of 32
-  const uint32_t chunk = ((n + size - 1) / size + kThreads - 1) / kThreads * kThreads;
+  // a CTA's slots, a multiple of its threads so that every warp has whole rows of 32
+  const uint32_t chunk = ((n + size - 1) / size + THREADS - 1) / THREADS * THREADS;
   const uint32_t lo = min(n, rank * chunk), hi = min(n, lo + chunk);
+  // Keys; and the weights and positions below the new length go out as they
+  // are (the second kernel writes over those of the holes).
+  const int64_t next = a.next ? int64_t(a.next[b]) : int64_t(n);
+  const bool w_copy = a.w_out != a.w_in, p_copy = a.p_out && a.p_out != a.p_in;
+  const uint32_t stop = leave ? hi : min(hi, w_copy || p_copy ? m : 0);
+  for (uint32_t i = tid; i < kBins; i += THREADS) s_bin[i] = 0;
+  __syncthreads();
+  for (uint32_t t0 = lo + tid; t0 < stop; t0 += 4 * THREADS) {
+    float wt[4];
+    int32_t pos[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t t = t0 + i * THREADS;
+      wt[i] = t < stop ? a.w_in[base + t] : 0.f;
+      pos[i] = a.p_in ? (t < stop ? a.p_in[base + t] : 0) : int32_t(t);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t t = t0 + i * THREADS;
+      if (t >= stop) break;
+      const bool held = pos[i] < int64_t(a.sink) || pos[i] >= next - int64_t(a.recent);
+      const uint32_t k = held ? kKeep : key_of(wt[i]);
+      s_key[t - lo] = k;
+      atomicAdd(&s_bin[k >> 21], 1u);
+      if (t < m && w_copy) a.w_out[base + t] = wt[i];
+      if (t < m && p_copy) a.p_out[base + t] = pos[i];
+    }
+  }
   if (leave == 0) {  // the same for the whole cluster
     if (rank == 0 && tid == 0) a.counts[row] = 0;
-    for (uint32_t t = lo + tid; t < hi; t += kThreads) {
-      if (a.w_out != a.w_in) a.w_out[base + t] = a.w_in[base + t];
-      if (a.p_out && a.p_out != a.p_in) a.p_out[base + t] = a.p_in ? a.p_in[base + t] : int32_t(t);
-    }
     return;
   }
-  const int64_t next = a.next ? int64_t(a.next[b]) : int64_t(n);
-  for (uint32_t t = lo + tid; t < hi; t += kThreads) {
-    const int64_t pos = a.p_in ? int64_t(a.p_in[base + t]) : int64_t(t);
-    const bool held = pos < int64_t(a.sink) || pos >= next - int64_t(a.recent);
-    s_key[t - lo] = held ? kKeep : key_of(a.w_in[base + t]);
-  }
-  // the leave-th smallest key, digit by digit; `want` counts within the keys that share the digits so far
-  uint32_t found = 0, mask = 0, want = leave;
+  // The leave-th smallest key, digit by digit; `want` counts within the keys
+  // that share the digits so far. Once all of them leave, their lower digits do not matter.
+  uint32_t found = 0, mask = 0, want = leave, same = 0;
   for (int digit = 0; digit < 3; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
     const uint32_t bins = digit == 2 ? 1024 : kBins;
-    for (uint32_t i = tid; i < bins; i += kThreads) s_bin[i] = 0;
-    __syncthreads();
-    for (uint32_t t = tid; t < hi - lo; t += kThreads) {
-      const uint32_t k = s_key[t];
-      if ((k & mask) == found) atomicAdd(&s_bin[(k >> shift) & (bins - 1)], 1u);
-    }
-    cluster_sync();
-    // two neighbouring bins a thread, summed over the cluster
-    uint32_t c0 = 0, c1 = 0;
-    if (2 * tid < bins)
-      for (uint32_t r = 0; r < size; ++r) {
-        c0 += peer_u32(&s_bin[2 * tid], r);
-        c1 += peer_u32(&s_bin[2 * tid + 1], r);
+    if (digit) {
+      for (uint32_t i = tid; i < kBins; i += THREADS) s_bin[i] = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (uint32_t t = tid; t < hi - lo; t += THREADS) {
+        const uint32_t k = s_key[t];
+        if ((k & mask) == found) atomicAdd(&s_bin[(k >> shift) & (bins - 1)], 1u);
       }
-    uint32_t total;
-    const uint32_t before = cta_prefix(c0 + c1, s_w, &total);
-    if (before < want && want <= before + c0) {
-      s_found[0] = 2 * tid;
-      s_found[1] = before;
-    } else if (before + c0 < want && want <= before + c0 + c1) {
-      s_found[0] = 2 * tid + 1;
-      s_found[1] = before + c0;
     }
-    cluster_sync();  // also: every CTA has read this one's bins
+    group_sync<CLUSTER>();
+    // neighbouring bins a thread, summed over the cluster
+    uint32_t c[kMine] = {}, sum = 0;
+    if constexpr (CLUSTER) {
+      uint32_t far[kMaxCluster][kMine];  // all on their way at once
+#pragma unroll
+      for (uint32_t r = 0; r < kMaxCluster; ++r) peer_bins<kMine>(far[r], &s_bin[kMine * tid], r, r < size);
+#pragma unroll
+      for (uint32_t r = 0; r < kMaxCluster; ++r)
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) c[i] += far[r][i];
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < kMine; ++i) c[i] = s_bin[kMine * tid + i];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) sum += c[i];
+    uint32_t total;
+    uint32_t before = cta_prefix<THREADS>(sum, s_w, &total);
+    if (before < want && want <= before + sum) {
+#pragma unroll
+      for (uint32_t i = 0; i < kMine; ++i) {
+        if (before < want && want <= before + c[i]) {
+          s_found[0] = kMine * tid + i;
+          s_found[1] = before;
+          s_found[2] = c[i];
+        }
+        before += c[i];
+      }
+    }
+    group_sync<CLUSTER>();  // also: every CTA has read this one's bins
     found |= s_found[0] << shift;
     mask |= (bins - 1) << shift;
     want -= s_found[1];
+    same = s_found[2];
+    if (same == want) break;  // the same in all threads of the cluster
   }
   // `want` of the keys equal to `found` leave, lowest slots first. A warp walks
   // its own run of consecutive slots.
   const uint32_t run = chunk / kWarps, w0 = min(hi, lo + w * run), w1 = min(hi, w0 + run);
   auto walk = [&](auto&& body) {
+#pragma unroll 4
     for (uint32_t t = w0; t < w1; t += 32) body(t + lane, t + lane < w1 ? s_key[t + lane - lo] : 0u, t + lane < w1);
   };
-  // number of v over the slots before this warp's, cluster-wide
+  // v summed over the warps before this one, cluster-wide
   auto before_warp = [&](uint32_t v, uint32_t* s_total, uint32_t* cluster_total) {
     uint32_t total;
-    const uint32_t mine = cta_prefix(lane == 0 ? v : 0u, s_w, &total);
-    if (tid == 0) *s_total = total;
-    cluster_sync();
-    uint32_t before = 0, all = 0;
-    for (uint32_t r = 0; r < size; ++r) {
-      const uint32_t x = peer_u32(s_total, r);
-      if (r < rank) before += x;
-      all += x;
+    const uint32_t mine = cta_prefix<THREADS>(lane == 0 ? v : 0u, s_w, &total);
+    uint32_t before = 0, all = total;
+    if constexpr (CLUSTER) {
+      if (tid == 0) *s_total = total;
+      group_sync<CLUSTER>();
+      all = 0;
+#pragma unroll
+      for (uint32_t r = 0; r < kMaxCluster; ++r) {
+        const uint32_t x = r < size ? peer_u32(s_total, r) : 0;
+        if (r < rank) before += x;
+        all += x;
+      }
     }
     *cluster_total = all;
     return before + __shfl_sync(0xffffffffu, mine, 0);
   };
-  uint32_t ties = 0, all;
-  walk([&](uint32_t, uint32_t k, bool in) { ties += __popc(__ballot_sync(0xffffffffu, in && k == found)); });
-  const uint32_t tie0 = before_warp(ties, &s_ties, &all);
-  const uint32_t below = (1u << lane) - 1;
-  uint32_t holes = 0, kept = 0, seen = tie0;
-  walk([&](uint32_t t, uint32_t k, bool in) {
+  // whether the lane's slot leaves; `seen`: equal keys before this row of slots
+  const bool all_same = want == same;
+  const uint32_t below = (1u << lane) - 1, limit = found | ~mask;  // all_same: everything up to `limit` leaves
+  uint32_t tie0 = 0, seen = 0, all;
+  auto leaves = [&](uint32_t k, bool in) {
+    if (all_same) return in && k <= limit;
     const uint32_t eq = __ballot_sync(0xffffffffu, in && k == found);
     const bool gone = in && (k < found || (k == found && seen + __popc(eq & below) < want));
     seen += __popc(eq);
+    return gone;
+  };
+  if (!all_same) {
+    uint32_t ties = 0;
+    walk([&](uint32_t, uint32_t k, bool in) { ties += __popc(__ballot_sync(0xffffffffu, in && k == found)); });
+    tie0 = before_warp(ties, &s_ties, &all);
+  }
+  uint32_t holes = 0, kept = 0;
+  seen = tie0;
+  walk([&](uint32_t t, uint32_t k, bool in) {
+    const bool gone = leaves(k, in);
     holes += __popc(__ballot_sync(0xffffffffu, gone && t < m));
     kept += __popc(__ballot_sync(0xffffffffu, in && !gone && t >= m));
   });
@@ -202,30 +282,27 @@ __global__ void __launch_bounds__(kThreads, 1) evict_select_kernel(const __grid_
   uint32_t hole0 = before_warp(holes, &s_moves[0], &moved);
   uint32_t kept0 = before_warp(kept, &s_moves[1], &all);
   seen = tie0;
-  uint2* list = a.moves + uint64_t(row) * a.room;
-  walk([&](uint32_t t, uint32_t k, bool in) {
-    const uint32_t eq = __ballot_sync(0xffffffffu, in && k == found);
-    const bool gone = in && (k < found || (k == found && seen + __popc(eq & below) < want));
-    seen += __popc(eq);
-    const bool hole = gone && t < m, mover = in && !gone && t >= m;
-    const uint32_t hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, mover);
-    if (hole) list[hole0 + __popc(hb & below)].y = t;
-    if (mover) list[kept0 + __popc(mb & below)].x = t;
-    hole0 += __popc(hb);
-    kept0 += __popc(mb);
-    if (in && !gone && t < m) {
-      if (a.w_out != a.w_in) a.w_out[base + t] = a.w_in[base + t];
-      if (a.p_out && a.p_out != a.p_in) a.p_out[base + t] = a.p_in ? a.p_in[base + t] : int32_t(t);
-    }
-  });
+  uint32_t *from = a.moves + uint64_t(row) * 2 * a.room, *to = from + a.room;
+  if (__any_sync(0xffffffffu, holes | kept)) {
+    walk([&](uint32_t t, uint32_t k, bool in) {
+      const bool gone = leaves(k, in);
+      const bool hole = gone && t < m, mover = in && !gone && t >= m;
+      const uint32_t hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, mover);
+      if (hole) to[hole0 + __popc(hb & below)] = t;
+      if (mover) from[kept0 + __popc(mb & below)] = t;
+      hole0 += __popc(hb);
+      kept0 += __popc(mb);
+    });
+  }
   if (rank == 0 && tid == 0) a.counts[row] = moved;
-  cluster_sync();  // no CTA leaves while another may still read its counts
+  if constexpr (CLUSTER) group_sync<CLUSTER>();  // no CTA leaves while another may still read its counts
 }
 
 // Kept slots from behind the new length into the holes below it: sources and
-// destinations do not meet, so the order is free. A thread moves 16 bytes of a
-// key or a value; `parts` of them make a slot.
-__global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ EvictArgs a, FastDiv parts) {
+// destinations do not meet, so the order is free. Eight lanes move a pair, each
+// up to four 16-byte pieces of its key and of its value, all in flight at once.
+constexpr uint32_t kLanes = 8;
+__global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ EvictArgs a) {
   const uint32_t row = blockIdx.y, b = row / a.kv.kv_heads, h = row - b * a.kv.kv_heads;
   pdl_launch_dependents();
   pdl_wait();
@@ -233,27 +310,44 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__
     const int32_t n = a.len_in[b];  // read and written by this thread alone
     a.len_out[b] = int32_t(min(n < 0 ? 0u : min(uint32_t(n), a.most), a.budget));
   }
-  const uint32_t moved = a.counts[row];
+  const uint32_t pairs = a.counts[row], chunks = a.kv.hd / 8, l = threadIdx.x % kLanes;
   const uint64_t base = uint64_t(row) * a.stride;
-  const uint2* list = a.moves + uint64_t(row) * a.room;
+  const uint32_t *froms = a.moves + uint64_t(row) * 2 * a.room, *tos = froms + a.room;
   const int32_t* pages = a.kv.pages + b * a.kv.pages_stride;
-  const uint32_t chunks = a.kv.hd / 8;
-  const uint64_t items = uint64_t(moved) * parts.d;
-  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < items; i += uint64_t(gridDim.x) * 256) {
-    const uint32_t pair = uint32_t(i / parts.d), part = uint32_t(i - uint64_t(pair) * parts.d);
-    const uint2 mv = list[pair];
+  uint16_t *k_pool = const_cast<uint16_t*>(a.kv.k), *v_pool = const_cast<uint16_t*>(a.kv.v);
+  for (uint32_t i = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes; i < pairs; i += gridDim.x * (256 / kLanes)) {
+    const uint2 mv = make_uint2(froms[i], tos[i]);
     const uint64_t from = paged_slot(a.kv, pages, mv.x, h), to = paged_slot(a.kv, pages, mv.y, h);
-    if (from == kNoCell || to == kNoCell) {
-      atomicOr(a.err, KERR_BAD_INDEX);
-    } else {
-      const bool is_v = part >= chunks;
-      const uint16_t* src = is_v ? a.kv.v : a.kv.k;
-      const uint32_t at = (is_v ? part - chunks : part) * 8;
-      *reinterpret_cast<uint4*>(const_cast<uint16_t*>(src) + to + at) = *reinterpret_cast<const uint4*>(src + from + at);
+    float w = 0.f;
+    int32_t p = 0;
+    if (l == 0) {
+      w = a.w_in[base + mv.x];
+      p = a.p_in ? a.p_in[base + mv.x] : int32_t(mv.x);
     }
-    if (part == 0) {
-      a.w_out[base + mv.y] = a.w_in[base + mv.x];
-      if (a.p_out) a.p_out[base + mv.y] = a.p_in ? a.p_in[base + mv.x] : int32_t(mv.x);
+    if (from != kNoCell && to != kNoCell) {
+      uint4 k[4], v[4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t ch = l + j * kLanes;
+        if (ch < chunks) {
+          k[j] = *reinterpret_cast<const uint4*>(k_pool + from + ch * 8);
+          v[j] = *reinterpret_cast<const uint4*>(v_pool + from + ch * 8);
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t ch = l + j * kLanes;
+        if (ch < chunks) {
+          *reinterpret_cast<uint4*>(k_pool + to + ch * 8) = k[j];
+          *reinterpret_cast<uint4*>(v_pool + to + ch * 8) = v[j];
+        }
+      }
+    } else if (l == 0) {
+      atomicOr(a.err, KERR_BAD_INDEX);
+    }
+    if (l == 0) {
+      a.w_out[base + mv.y] = w;
+      if (a.p_out) a.p_out[base + mv.y] = p;
     }
   }
 }
@@ -262,7 +356,17 @@ uint64_t rows_of(const si_paged_kv& kv) { return uint64_t(kv.sequences) * kv.kv_
 // A list holds at most half of the slots: one of a pair is below the budget, one behind it.
 uint64_t room_of(const si_paged_kv& kv) { return uint64_t(kv.max_pages) * kv.page_tokens / 2 + 1; }
 uint64_t evict_bytes(const si_paged_kv& kv) {
-  return ((rows_of(kv) * 4 + 15) & ~uint64_t(15)) + rows_of(kv) * room_of(kv) * sizeof(uint2);
+  return ((rows_of(kv) * 4 + 15) & ~uint64_t(15)) + rows_of(kv) * room_of(kv) * 8;
+}
+
+template <int THREADS, bool CLUSTER>
+cudaError_t select(const EvictArgs& p, uint32_t rows, uint32_t cluster, uint32_t each, cudaStream_t s) {
+  static std::atomic<uint32_t> cache[kMaxDevices];
+  const uint32_t bytes = (each + THREADS - 1) / THREADS * THREADS * 4;
+  if (cudaError_t e = raise_smem_limit(evict_select_kernel<THREADS, CLUSTER>, bytes, cache)) return e;
+  PdlLaunch l(dim3(rows * cluster), dim3(THREADS), bytes, s);
+  if (CLUSTER) l.cluster(cluster);
+  return cudaLaunchKernelEx(&l.cfg, evict_select_kernel<THREADS, CLUSTER>, p);
 }
 
 int check_size(const si_paged_kv* kv, std::string* msg) {
@@ -328,24 +432,28 @@ extern "C" int si_paged_evict_dev(si_ctx* ctx, const si_paged_kv* kv, const si_p
   p.most = uint32_t(std::min<uint64_t>(p.kv.max_tokens, a->weights_stride));
   p.room = uint32_t(room_of(*kv));
   p.counts = static_cast<uint32_t*>(a->work);
-  p.moves = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a->work) + ((rows_of(*kv) * 4 + 15) & ~uint64_t(15)));
+  p.moves = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a->work) + ((rows_of(*kv) * 4 + 15) & ~uint64_t(15)));
   p.err = ctx->d_err;
   const cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   const uint32_t rows = uint32_t(rows_of(*kv)), most = p.most;
+  // A CTA for 8192 keys, as long as the clusters find room beside each other: a
+  // graphics processing cluster has 14 multiprocessors or more, so 8 of them
+  // hold 8, 24 or 56 clusters of 8, 4 or 2 CTAs for sure. (16 rows of 131,072: a
+  // second wave of clusters of 8 cost 35 us.)
   uint32_t cluster = 1;
-  while (cluster < kMaxCluster && most > cluster * 8192) cluster *= 2;
-  const uint32_t slots = ((most + cluster - 1) / cluster + kThreads - 1) / kThreads * kThreads;
-  static std::atomic<uint32_t> cache[kMaxDevices];
-  if (cudaError_t e = raise_smem_limit(evict_select_kernel, slots * 4, cache)) return cuda_fail(ctx, e, "paged eviction");
-  PdlLaunch l(dim3(rows * cluster), dim3(kThreads), slots * 4, s);
-  l.cluster(cluster);
-  if (cudaError_t e = cudaLaunchKernelEx(&l.cfg, evict_select_kernel, p)) return cuda_fail(ctx, e, "paged eviction launch");
-  const FastDiv parts = fast_div(2 * (kv->head_dim / 8));
+  while (cluster < kMaxCluster && most > cluster * 8192 &&
+         (most > cluster * kCtaSlots || rows <= (cluster == 1 ? 56u : cluster == 2 ? 24u : 8u)))
+    cluster *= 2;
+  const uint32_t each = (most + cluster - 1) / cluster;
+  // 256, 512 or 1024 threads for about 16 keys a thread
+  const cudaError_t e = cluster > 1 ? (each > 8192 ? select<1024, true>(p, rows, cluster, each, s) : select<512, true>(p, rows, cluster, each, s))
+                        : each > 8192 ? select<1024, false>(p, rows, 1, each, s) : each > 2048 ? select<512, false>(p, rows, 1, each, s) : select<256, false>(p, rows, 1, each, s);
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "paged eviction launch");
   // moves of one row are at most the smaller of both sides of the budget
-  const uint64_t items = std::min<uint64_t>(most > a->budget ? most - a->budget : 0, a->budget) * parts.d;
-  const uint32_t wide = std::max(1u, uint32_t(ctx->sm_count) * 8 / rows);
-  PdlLaunch v(dim3(uint32_t(std::max<uint64_t>(1, std::min<uint64_t>((items + 255) / 256, wide))), rows), dim3(256), 0, s);
-  if (cudaError_t e = cudaLaunchKernelEx(&v.cfg, evict_move_kernel, p, parts)) return cuda_fail(ctx, e, "paged eviction launch");
+  const uint64_t lanes = std::min<uint64_t>(most > a->budget ? most - a->budget : 0, a->budget) * kLanes;
+  const uint32_t wide = std::max(1u, uint32_t(ctx->sm_count) * 16 / rows);
+  PdlLaunch v(dim3(uint32_t(std::max<uint64_t>(1, std::min<uint64_t>((lanes + 255) / 256, wide))), rows), dim3(256), 0, s);
+  if (cudaError_t e = cudaLaunchKernelEx(&v.cfg, evict_move_kernel, p)) return cuda_fail(ctx, e, "paged eviction launch");
   note_async_submission(ctx);
   return SI_OK;
 }
