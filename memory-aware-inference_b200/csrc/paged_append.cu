@@ -7,12 +7,15 @@
 // turn is exact to 2^-33 turns for any 32-bit position, where p * f in f32 is
 // off by 0.03 rad at position 500,000. sincospif of the top 32 bits as a
 // fraction of a half turn finishes it.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace si {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr uint32_t kMaxTokens = 8;  // of a CTA
 
 struct AppendArgs {
   PagedView kv;
@@ -22,127 +25,181 @@ struct AppendArgs {
   const int32_t *sequence, *slot, *position;
   const uint64_t* rope;
   float rope_scale;
-  uint32_t elem, cache_elem, tokens, qh, kvh, half, interleaved;
+  uint32_t tokens, kvh, half, interleaved;
   uint32_t per_cta;      // tokens of a CTA
-  uint32_t rot_slots;    // threads of a head that rotate
-  FastDiv slots, heads;  // threads of a head; heads of a token (q, k, v)
+  uint32_t rot_parts;    // parts of a head that rotate
+  FastDiv parts;         // parts of a head, a thread each
+  FastDiv q_heads, kv_heads;
   int* err;
 };
 
 // One thread's part of a head: VEC pairs (two runs of VEC elements in the half
-// layout, one run of 2 VEC neighbouring elements in the interleaved one) or, past the rotated
-// dims, a run to copy.
+// layout, one run of 2 VEC neighbouring elements in the interleaved one) or,
+// past the rotated dims, a run to copy.
 //
-// Bandwidth bound: every element is read once and written once. A CTA takes a
-// few tokens, makes their sines once in shared memory, and walks the (token,
-// head, run) items of all three inputs, so that heads share the sines and the
-// accesses of a warp are contiguous.
-template <int VEC>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
-  extern __shared__ float2 s_turn[];  // [per_cta][half] (cos, sin)
+// Bandwidth bound: every element is read once and written once, and what there
+// is to gain is few instructions in between. A CTA takes a few tokens and makes
+// their sines and their places in the cache once in shared memory. A thread
+// keeps its part of a head and walks the rows (token, head) of the queries,
+// then of the keys, then of the values, in batches whose loads are all on their way
+// before the first is used. Sines lie so that neighbouring parts read
+// neighbouring banks.
+template <int VEC, uint32_t ELEM>
+struct Run {  // VEC elements as they lie in memory
+  static constexpr int kRegs = VEC == 8 ? (ELEM == SI_ELEM_F32 ? 8 : 4) : 1;
+  uint32_t r[kRegs];
+  __device__ __forceinline__ void load(const void* p, uint64_t i) {
+    if constexpr (VEC == 8) {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * elem_bytes(ELEM));
+#pragma unroll
+      for (int j = 0; j < kRegs / 4; ++j) {
+        const uint4 v = q[j];
+        r[4 * j] = v.x, r[4 * j + 1] = v.y, r[4 * j + 2] = v.z, r[4 * j + 3] = v.w;
+      }
+    } else if constexpr (ELEM == SI_ELEM_F32) {
+      r[0] = static_cast<const uint32_t*>(p)[i];
+    } else {
+      r[0] = static_cast<const uint16_t*>(p)[i];
+    }
+  }
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (ELEM == SI_ELEM_F32) return __uint_as_float(r[j]);
+    return elem_to_f(uint16_t(r[j / 2] >> (j % 2 * 16)), ELEM);
+  }
+};
+template <int VEC, uint32_t ELEM>
+__device__ __forceinline__ void store_run(void* p, uint64_t i, const float x[VEC]) {
+  if constexpr (VEC == 8) {
+    store8(p, i, ELEM, true, x);
+  } else if constexpr (ELEM == SI_ELEM_F32) {
+    static_cast<float*>(p)[i] = x[0];
+  } else {
+    static_cast<uint16_t*>(p)[i] = f_to_elem(x[0], ELEM);
+  }
+}
+
+enum Kind { kQuery, kKey, kValue };
+
+template <int VEC, uint32_t ELEM, uint32_t CACHE>
+__global__ void __launch_bounds__(kThreads, 4) append_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int kBatch = 2;  // more would spill: 4 rows at once took 47 us where 2 take 37 (8192 tokens, 32 + 8 + 8 heads of 128)
+  extern __shared__ float2 s_turn[];  // [per_cta][VEC][rotating parts] (cos, sin)
+  __shared__ uint64_t s_cell[kMaxTokens];
+  __shared__ int32_t s_slot[kMaxTokens];
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t t0 = blockIdx.x * a.per_cta, nt = min(a.per_cta, a.tokens - t0);
+  if (threadIdx.x < nt) {
+    const uint32_t tok = t0 + threadIdx.x;
+    const int32_t slot = a.slot[tok];
+    uint64_t cell = kNoCell;
+    if (slot >= 0 && a.kvh) {
+      const uint32_t b = a.sequence ? uint32_t(a.sequence[tok]) : tok;
+      if (b < a.kv.sequences && uint32_t(slot) < a.kv.max_tokens)
+        cell = paged_slot(a.kv, a.kv.pages + b * a.kv.pages_stride, uint32_t(slot), 0);
+      if (cell == kNoCell) atomicOr(a.err, KERR_BAD_INDEX);
+    }
+    s_slot[threadIdx.x] = slot;
+    s_cell[threadIdx.x] = cell;
+  }
   for (uint32_t i = threadIdx.x; i < nt * a.half; i += kThreads) {
     const uint32_t t = i / a.half, j = i - t * a.half;
     const int32_t pos = a.position ? a.position[t0 + t] : a.slot[t0 + t];
     // two's complement: a negative position turns the other way
     const uint64_t turn = uint64_t(int64_t(pos)) * a.rope[j];
-    const float x = float(int32_t(uint32_t(turn >> 32))) * 0x1p-31f;  // half turns, in [-1, 1]
+    const float half_turns = float(int32_t(uint32_t(turn >> 32))) * 0x1p-31f;  // in [-1, 1]
     float s, c;
-    sincospif(x, &s, &c);
-    s_turn[i] = make_float2(c * a.rope_scale, s * a.rope_scale);
+    sincospif(half_turns, &s, &c);
+    s_turn[t * a.half + j % VEC * a.rot_parts + j / VEC] = make_float2(c * a.rope_scale, s * a.rope_scale);
   }
   __syncthreads();
-  const uint32_t rows = nt * a.heads.d, items = rows * a.slots.d;
-  for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
-    const uint32_t row = div_of(i, a.slots), part = i - row * a.slots.d;
-    const uint32_t t = div_of(row, a.heads), head = row - t * a.heads.d, tok = t0 + t;
-    const int32_t slot = a.slot[tok];
-    if (slot < 0) continue;  // padding
-    const bool is_q = head < a.qh, is_k = !is_q && head < a.qh + a.kvh;
-    const uint32_t h = is_q ? head : is_k ? head - a.qh : head - a.qh - a.kvh;
-    const void* src = is_q ? a.q : is_k ? a.k : a.v;
-    const uint64_t from = is_q ? tok * a.q_ts + h * a.q_hs : is_k ? tok * a.k_ts + h * a.k_hs : tok * a.v_ts + h * a.v_hs;
-    uint64_t to;
-    void* dst;
-    uint32_t elem;
-    if (is_q) {
-      to = tok * a.qo_ts + h * a.qo_hs;
-      dst = a.q_out;
-      elem = a.elem;
-    } else {
-      const uint32_t b = a.sequence ? uint32_t(a.sequence[tok]) : tok;
-      to = kNoCell;
-      if (b < a.kv.sequences && uint32_t(slot) < a.kv.max_tokens)
-        to = paged_slot(a.kv, a.kv.pages + b * a.kv.pages_stride, uint32_t(slot), h);
-      if (to == kNoCell) {
-        atomicOr(a.err, KERR_BAD_INDEX);
-        continue;
-      }
-      dst = const_cast<uint16_t*>(is_k ? a.kv.k : a.kv.v);
-      elem = a.cache_elem;
-    }
-    // dims of the two runs; a value head copies all of its runs
-    uint32_t d0, d1;
-    bool turn = part < a.rot_slots;
-    if (turn) {
-      d0 = a.interleaved ? part * 2 * VEC : part * VEC;
-      d1 = a.interleaved ? d0 + VEC : d0 + a.half;
-    } else {
-      d0 = 2 * a.half + (part - a.rot_slots) * 2 * VEC;
-      d1 = d0 + VEC;
-    }
-    const bool second = d1 < a.kv.hd;  // the last copied run may be single
-    float x[VEC], y[VEC];
-    if constexpr (VEC == 8) {
-      load8(src, from + d0, a.elem, true, x);
-      if (second) load8(src, from + d1, a.elem, true, y);
-    } else {
-      if (a.elem == SI_ELEM_F32) {
-        x[0] = static_cast<const float*>(src)[from + d0];
-        y[0] = second ? static_cast<const float*>(src)[from + d1] : 0.f;
-      } else {
-        x[0] = elem_to_f(static_cast<const uint16_t*>(src)[from + d0], a.elem);
-        y[0] = second ? elem_to_f(static_cast<const uint16_t*>(src)[from + d1], a.elem) : 0.f;
-      }
-    }
-    if (turn && (is_q || is_k)) {
-      const float2* cs = s_turn + t * a.half;
-      if (VEC == 8 && a.interleaved) {
-#pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
-          const float2 u = cs[(d0 + j) / 2], w = cs[(d1 + j) / 2];
-          const float x0 = x[j], x1 = x[j + 1 < VEC ? j + 1 : j], y0 = y[j], y1 = y[j + 1 < VEC ? j + 1 : j];
-          x[j] = x0 * u.x - x1 * u.y;
-          x[j + 1 < VEC ? j + 1 : j] = x0 * u.y + x1 * u.x;
-          y[j] = y0 * w.x - y1 * w.y;
-          y[j + 1 < VEC ? j + 1 : j] = y0 * w.y + y1 * w.x;
-        }
-      } else {
-        const uint32_t p0 = a.interleaved ? d0 / 2 : d0;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float2 u = cs[p0 + j];
-          const float x0 = x[j], y0 = y[j];
-          x[j] = x0 * u.x - y0 * u.y;
-          y[j] = x0 * u.y + y0 * u.x;
-        }
-      }
-    }
-    if constexpr (VEC == 8) {
-      store8(dst, to + d0, elem, true, x);
-      if (second) store8(dst, to + d1, elem, true, y);
-    } else {
-      if (elem == SI_ELEM_F32) {
-        static_cast<float*>(dst)[to + d0] = x[0];
-        if (second) static_cast<float*>(dst)[to + d1] = y[0];
-      } else {
-        static_cast<uint16_t*>(dst)[to + d0] = f_to_elem(x[0], elem);
-        if (second) static_cast<uint16_t*>(dst)[to + d1] = f_to_elem(y[0], elem);
-      }
-    }
+  const uint32_t row0 = div_of(threadIdx.x, a.parts), part = threadIdx.x - row0 * a.parts.d, rows_at_once = kThreads / a.parts.d;
+  if (row0 >= rows_at_once) return;
+  const bool rotates = part < a.rot_parts;
+  // dims of the two runs; the second may be missing in the last copied part
+  uint32_t d0, d1;
+  if (rotates) {
+    d0 = a.interleaved ? part * 2 * VEC : part * VEC;
+    d1 = a.interleaved ? d0 + VEC : d0 + a.half;
+  } else {
+    d0 = 2 * a.half + (part - a.rot_parts) * 2 * VEC;
+    d1 = d0 + VEC;
   }
+  const bool second = d1 < a.kv.hd;
+
+  auto walk = [&](auto kind, const void* src, uint64_t ts, uint64_t hs, const FastDiv& heads) {
+    constexpr Kind K = decltype(kind)::value;
+    const uint32_t rows = nt * heads.d;
+    for (uint32_t r0 = row0; r0 < rows; r0 += kBatch * rows_at_once) {
+      Run<VEC, ELEM> x[kBatch], y[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const uint32_t r = r0 + j * rows_at_once, t = div_of(r, heads), h = r - t * heads.d;
+        if (r >= rows) continue;
+        const uint64_t from = uint64_t(t0 + t) * ts + h * hs;
+        x[j].load(src, from + d0);
+        if (second) y[j].load(src, from + d1);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const uint32_t r = r0 + j * rows_at_once, t = div_of(r, heads), h = r - t * heads.d;
+        if (r >= rows || s_slot[t] < 0) continue;  // past the end, or padding
+        float u[VEC], w[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) u[e] = x[j].at(e), w[e] = y[j].at(e);
+        if (K != kValue && rotates) {
+          float2 f[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) f[e] = s_turn[t * a.half + e * a.rot_parts + part];
+          if (VEC == 8 && a.interleaved) {  // pairs side by side: the first four in u, the others in w
+#pragma unroll
+            for (int e = 0; e < VEC / 2; ++e) {
+              const float u0 = u[2 * e], u1 = u[2 * e + 1], w0 = w[2 * e], w1 = w[2 * e + 1];
+              const float2 g = f[e], k = f[VEC / 2 + e];
+              u[2 * e] = u0 * g.x - u1 * g.y;
+              u[2 * e + 1] = u0 * g.y + u1 * g.x;
+              w[2 * e] = w0 * k.x - w1 * k.y;
+              w[2 * e + 1] = w0 * k.y + w1 * k.x;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const float u0 = u[e], w0 = w[e];
+              u[e] = u0 * f[e].x - w0 * f[e].y;
+              w[e] = u0 * f[e].y + w0 * f[e].x;
+            }
+          }
+        }
+        if constexpr (K == kQuery) {
+          const uint64_t to = uint64_t(t0 + t) * a.qo_ts + h * a.qo_hs;
+          store_run<VEC, ELEM>(a.q_out, to + d0, u);
+          if (second) store_run<VEC, ELEM>(a.q_out, to + d1, w);
+        } else if (s_cell[t] != kNoCell) {
+          uint16_t* dst = const_cast<uint16_t*>(K == kKey ? a.kv.k : a.kv.v);
+          const uint64_t to = s_cell[t] + uint64_t(h) * a.kv.head_stride;
+          store_run<VEC, CACHE>(dst, to + d0, u);
+          if (second) store_run<VEC, CACHE>(dst, to + d1, w);
+        }
+      }
+    }
+  };
+  if (a.q_heads.d) walk(std::integral_constant<Kind, kQuery>(), a.q, a.q_ts, a.q_hs, a.q_heads);
+  if (a.kvh) {
+    walk(std::integral_constant<Kind, kKey>(), a.k, a.k_ts, a.k_hs, a.kv_heads);
+    walk(std::integral_constant<Kind, kValue>(), a.v, a.v_ts, a.v_hs, a.kv_heads);
+  }
+}
+
+template <int VEC, uint32_t ELEM>
+cudaError_t launch(const cudaLaunchConfig_t* cfg, const AppendArgs& p, uint32_t cache) {
+  return cache == SI_ELEM_BF16 ? cudaLaunchKernelEx(cfg, append_kernel<VEC, ELEM, SI_ELEM_BF16>, p)
+                               : cudaLaunchKernelEx(cfg, append_kernel<VEC, ELEM, SI_ELEM_F16>, p);
+}
+template <int VEC>
+cudaError_t launch(const cudaLaunchConfig_t* cfg, const AppendArgs& p, uint32_t elem, uint32_t cache) {
+  return elem == SI_ELEM_F32    ? launch<VEC, SI_ELEM_F32>(cfg, p, cache)
+         : elem == SI_ELEM_BF16 ? launch<VEC, SI_ELEM_BF16>(cfg, p, cache)
+                                : launch<VEC, SI_ELEM_F16>(cfg, p, cache);
 }
 
 int check_append(const si_paged_kv* kv, const si_paged_append* a, std::string* msg) {
@@ -197,9 +254,9 @@ extern "C" int si_paged_append_dev(si_ctx* ctx, const si_paged_kv* kv, const si_
   p.sequence = a->sequence, p.slot = a->slot, p.position = a->position;
   p.rope = a->rope;
   p.rope_scale = a->rope_scale;
-  p.elem = a->elem, p.cache_elem = kv->elem;
   p.tokens = a->tokens;
-  p.qh = a->q ? a->query_heads : 0;
+  if (a->q) p.q_heads = fast_div(a->query_heads);
+  if (a->k) p.kv_heads = fast_div(kv->kv_heads);
   p.kvh = a->k ? kv->kv_heads : 0;
   p.half = a->rotary_dim / 2;
   p.interleaved = a->rope_layout == SI_ROPE_INTERLEAVED;
@@ -210,16 +267,15 @@ extern "C" int si_paged_append_dev(si_ctx* ctx, const si_paged_kv* kv, const si_
     wide = wide && wide_ok(a->q, a->elem, p.q_ts, p.q_hs) && wide_ok(a->q_out, a->elem, p.qo_ts, p.qo_hs);
   if (a->k) wide = wide && wide_ok(a->k, a->elem, p.k_ts, p.k_hs) && wide_ok(a->v, a->elem, p.v_ts, p.v_hs);
   const uint32_t vec = wide ? 8 : 1;
-  p.rot_slots = p.half / vec;
+  p.rot_parts = p.half / vec;
   const uint32_t rest = kv->head_dim - a->rotary_dim;
-  p.slots = fast_div(p.rot_slots + (rest + 2 * vec - 1) / (2 * vec));
-  p.heads = fast_div(p.qh + 2 * p.kvh);
+  p.parts = fast_div(p.rot_parts + (rest + 2 * vec - 1) / (2 * vec));
   // a CTA takes up to 8 tokens, fewer while that leaves multiprocessors without work
   p.per_cta = 1;
-  while (p.per_cta < 8 && p.tokens / (2 * p.per_cta) >= uint32_t(ctx->sm_count) * 4) p.per_cta *= 2;
+  while (p.per_cta < kMaxTokens && p.tokens / (2 * p.per_cta) >= uint32_t(ctx->sm_count) * 4) p.per_cta *= 2;
   const cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   PdlLaunch l(dim3((p.tokens + p.per_cta - 1) / p.per_cta), dim3(kThreads), size_t(p.per_cta) * p.half * sizeof(float2), s);
-  const cudaError_t e = wide ? cudaLaunchKernelEx(&l.cfg, append_kernel<8>, p) : cudaLaunchKernelEx(&l.cfg, append_kernel<1>, p);
+  const cudaError_t e = wide ? launch<8>(&l.cfg, p, a->elem, kv->elem) : launch<1>(&l.cfg, p, a->elem, kv->elem);
   if (e != cudaSuccess) return cuda_fail(ctx, e, "paged append launch");
   note_async_submission(ctx);
   return SI_OK;
