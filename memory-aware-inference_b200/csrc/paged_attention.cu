@@ -239,6 +239,8 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
   // per warp: [query terms, later the partial of the last pair][partial of the first pair]
   __shared__ uint32_t s_warp[NW];
   __shared__ Place s_part[2 * NW];  // pairs of the warps' partials; tiles 0: no partial
+  __shared__ uint8_t s_list[32], s_lead[32];
+  __shared__ uint32_t s_leads;
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + NW * kRegion);
   const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5, n8 = lane >> 2, c4 = lane & 3;
   const uint32_t heads = a.kv.kv_heads * a.blocks;
@@ -266,23 +268,6 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
   }
   const Shares cta_share(steps, ctas), warp_share(steps, ctas * NW);
   const uint32_t cu0 = cta_share.begin(cta), cu1 = cta_share.begin(cta + 1);
-  if (threadIdx.x == NW * 32 - 1) {
-    Join j = {-1, 0, 0, 0};
-    if (cta > 0) {
-      const Place p = place_of(cu0, prefix, a.kv.sequences, heads);
-      const uint32_t first = p.begin + kPairCost, end = first + p.tiles, before = cta_share.begin(cta - 1);
-      if (first < cu0 && (before <= first)) {  // the first border among this pair's units
-        j.slot0 = p.begin <= before ? 0 : 1;
-        uint32_t last = cta;
-        for (uint32_t step = 128; step; step >>= 1)  // whose share holds step end - 1
-          if (last + step < ctas && cta_share.begin(last + step) < end) last += step;
-        j.last = int32_t(last);
-        j.b = p.b;
-        j.head = p.head;
-      }
-    }
-    a.join[cta] = j;
-  }
   const uint32_t u0 = warp_share.begin(cta * NW + w), u1 = warp_share.begin(cta * NW + w + 1);
   float* region = smem + w * kRegion;
   uint4* s_q = reinterpret_cast<uint4*>(region) + lane;  // [step][term][lane]: a lane reads what it wrote
@@ -426,9 +411,9 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     for (uint32_t tile = t_begin; tile < t_end; ++tile) {
       const int32_t page_after = page_of(tile + 2);
-      // The leading terms in two chains, the small ones in a third: shorter
-      // chains of dependent products, and fewer roundings of a large sum.
-      float s[4] = {}, s_odd[4] = {}, s_low[4] = {};
+      // Several chains of dependent products, two a term: shorter ones, fewer
+      // roundings of a large sum, and small terms are not lost in large ones.
+      float s[4] = {}, chain[2 * TQ - 1][4] = {};
 #pragma unroll
       for (int st = 0; st < KK; ++st) {
         const uint4 x = kr[0][st], y = kr[1][st];
@@ -436,12 +421,17 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
 #pragma unroll
         for (int t = 0; t < TQ; ++t) {
           const uint4 qv = s_q[(st * TQ + t) * 32];
-          mma16<BF16>(t ? s_low : s, a0, qv.x, qv.y);
-          mma16<BF16>(t ? s_low : s_odd, a1, qv.z, qv.w);
+          mma16<BF16>(t ? chain[2 * t - 1] : s, a0, qv.x, qv.y);
+          mma16<BF16>(chain[2 * t], a1, qv.z, qv.w);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] += s_odd[i] + (TQ > 1 ? s_low[i] : 0.f);
+      for (int i = 0; i < 4; ++i) {
+        float low = 0.f;
+#pragma unroll
+        for (int t = TQ - 1; t > 0; --t) low += chain[2 * t - 1][i] + chain[2 * t][i];
+        s[i] += chain[0][i] + low;
+      }
       const bool lo_now = lo, hi_now = hi;
       cell = cell_of(tile + 1, page_next);
       page_next = page_after;
@@ -554,36 +544,65 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
     }
     __syncwarp();
   }
+  if (threadIdx.x == 0) {
+    Join j = {-1, 0, 0, 0};
+    if (cta > 0) {
+      const Place p = place_of(cu0, prefix, a.kv.sequences, heads);
+      const uint32_t first = p.begin + kPairCost, end = first + p.tiles, before = cta_share.begin(cta - 1);
+      if (first < cu0 && (before <= first)) {  // the first border among this pair's units
+        j.slot0 = p.begin <= before ? 0 : 1;
+        uint32_t last = cta;
+        for (uint32_t step = 128; step; step >>= 1)  // whose share holds step end - 1
+          if (last + step < ctas && cta_share.begin(last + step) < end) last += step;
+        j.last = int32_t(last);
+        j.b = p.b;
+        j.head = p.head;
+      }
+    }
+    a.join[cta] = j;
+  }
   __syncthreads();
-  // Join the warps' partials in the order of their units: partial e leads its
-  // pair if the one before it is of another pair, and the lead's outputs are
-  // shared out over all threads together with those of the other leads.
+  // Join the warps' partials in the order of their units. Warp 0 lists them:
+  // s_list[k] is the k-th partial, s_lead[i] the first one of the i-th pair.
+  if (w == 0) {
+    const Place p = s_part[lane < 2 * NW ? lane : 0];
+    const bool on = lane < 2 * NW && p.tiles != 0;
+    const uint32_t all = __ballot_sync(0xffffffffu, on), below = all & ((1u << lane) - 1);
+    const uint32_t before = __shfl_sync(0xffffffffu, p.begin, below ? 31 - __clz(below) : 0);
+    const uint32_t leads = __ballot_sync(0xffffffffu, on && (!below || before != p.begin));
+    if (on) s_list[__popc(below)] = uint8_t(lane);
+    if (leads >> lane & 1) s_lead[__popc(leads & ((1u << lane) - 1))] = uint8_t(__popc(below));
+    if (lane == 0) {
+      s_leads = __popc(leads);
+      s_lead[__popc(leads)] = uint8_t(__popc(all));
+    }
+  }
+  __syncthreads();
   constexpr uint32_t kItems = kCols * (HD / 8);
-  for (uint32_t i = threadIdx.x; i < 2 * NW * kItems; i += NW * 32) {
-    const uint32_t e = i / kItems, col = i % kItems / (HD / 8), ch = i % (HD / 8);
-    const Place at = s_part[e];
-    if (at.tiles == 0) continue;
-    uint32_t before = e;  // the nearest partial before e
-    while (before > 0 && s_part[before - 1].tiles == 0) --before;
-    if (before > 0 && s_part[before - 1].begin == at.begin) continue;
+  auto part_of = [&](uint32_t k) {
+    const uint32_t x = s_list[k];
+    return smem + (x / 2) * kRegion + (x % 2 ? 0 : kRegion - kPart);
+  };
+  for (uint32_t i = threadIdx.x; i < s_leads * kItems; i += NW * 32) {
+    const uint32_t g = i / kItems, col = i % kItems / (HD / 8), ch = i % (HD / 8);
+    const uint32_t k0 = s_lead[g], k1 = s_lead[g + 1];
+    const Place at = s_part[s_list[k0]];
     const uint32_t kvh = at.head / a.blocks, col0 = (at.head - kvh * a.blocks) * kCols;
     const uint32_t cols = min(kCols, a.group - col0), qhead0 = kvh * a.group + col0;
     if (col >= cols) continue;
     float m = -INFINITY, l = 0.f, o[8] = {};
-    for (uint32_t x = e; x < 2 * NW; ++x) {
-      if (s_part[x].tiles == 0) continue;
-      if (s_part[x].begin != at.begin) break;
-      const float* from = smem + (x / 2) * kRegion + (x % 2 ? 0 : kRegion - kPart);
+    for (uint32_t k = k0; k < k1; ++k) m = fmaxf(m, part_of(k)[kCols * HD + 2 * col]);
+#pragma unroll 4
+    for (uint32_t k = k0; k < k1; ++k) {
+      const float* from = part_of(k);
       const float2 ml = *reinterpret_cast<const float2*>(from + kCols * HD + 2 * col);
-      if (ml.x == -INFINITY) continue;
-      const float g = fmaxf(m, ml.x), f0 = exp2f(m - g), f1 = exp2f(ml.x - g);
-      m = g;
-      l = l * f0 + ml.y * f1;
+      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+      l += ml.y * f;
       const float4 v0 = *reinterpret_cast<const float4*>(from + col * HD + ch * 8);
       const float4 v1 = *reinterpret_cast<const float4*>(from + col * HD + ch * 8 + 4);
       const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = o[j] * f0 + v[j] * f1;
+      for (int j = 0; j < 8; ++j) o[j] += v[j] * f;
     }
     const uint32_t first = at.begin + kPairCost;
     if (first >= cu0 && first + at.tiles <= cu1) {

@@ -11,10 +11,13 @@
 // formed and summed in f64; two sums of different order differ by 1e-16, so
 // they choose differently about once in 10^10 draws.
 //
-// Two kernels: every CTA of the first decides the sequence's accepted count for
-// itself (a few loads) and sums one chunk of the row; one CTA a sequence of the second
-// scans the chunk sums, finds the chunk that the draw falls in, and scans
-// that chunk. The row is read once, one chunk of it twice.
+// Two kernels. Every warp of the first decides the sequence's accepted count
+// for itself (a few loads) and sums chunks of 512 tokens of the row, no barrier;
+// one CTA a sequence of the second scans the chunk sums, finds the chunk that
+// the draw falls in, and scans that chunk. The row is read once, one chunk of
+// it twice. A difference is max(p - q, 0) = p - min(p, q), so that the minimum is
+// taken in f32 and only the subtraction and the sum in f64: conversions have an eighth
+// of the f32 rate and were what bound the sums at first.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -24,7 +27,7 @@
 namespace si {
 namespace {
 
-constexpr uint32_t kThreads = 256, kEach = 16, kChunk = kThreads * kEach;  // tokens of a chunk
+constexpr uint32_t kThreads = 256, kEach = 16, kChunk = 32 * kEach;  // tokens of a chunk
 constexpr uint32_t kPickThreads = 1024;
 
 struct VerifyArgs {
@@ -34,26 +37,59 @@ struct VerifyArgs {
   const float *u, *u_last;
   int32_t *accepted, *next;
   uint32_t drafts, vocab, chunks;
-  double2* sums;  // [sequence][chunk]: of the difference, of the target's row
+  double* sums;  // [sequence][chunk]
   int* err;
 };
 
-__device__ __forceinline__ double weight_of(float x) {
-  return x > 0.f && x < INFINITY ? double(x) : 0.0;  // NaN compares false
-}
+// Negative, infinite and NaN entries count as 0 (NaN compares false).
+__device__ __forceinline__ float weight_of(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
 
 // The row that the next token is drawn from.
 struct Rest {
   const float* p;
   const float* q;     // null: nothing is taken away
   uint32_t without;   // this token's weight is taken away; >= vocab: none
-  __device__ __forceinline__ double at(uint32_t j, double* plain) const {
-    const double x = weight_of(p[j]);
-    *plain = x;
-    if (q) return fmax(x - weight_of(q[j]), 0.0);
-    return j == without ? 0.0 : x;
+  __device__ __forceinline__ double at(uint32_t j) const {
+    const float x = weight_of(p[j]);
+    if (q) return double(x) - double(fminf(x, weight_of(q[j])));
+    return j == without ? 0.0 : double(x);
   }
 };
+
+__device__ __forceinline__ float load_stream(const float* p) {
+  float x;
+  asm volatile("ld.global.nc.L1::no_allocate.f32 %0, [%1];" : "=f"(x) : "l"(p));
+  return x;
+}
+
+// Sum of chunk c by one warp, the same in all lanes. All loads are on their way
+// before the first value is used.
+__device__ __forceinline__ double chunk_sum(const Rest& r, uint32_t c, uint32_t vocab, uint32_t lane) {
+  const uint32_t j0 = c * kChunk + lane;
+  double s = 0.0;
+  float x[kEach], y[kEach];
+  if (c * kChunk + kChunk <= vocab) {
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) x[i] = load_stream(r.p + j0 + i * 32);
+    if (r.q) {
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i) y[i] = load_stream(r.q + j0 + i * 32);
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i) {
+        const float w = weight_of(x[i]);
+        s += double(w) - double(fminf(w, weight_of(y[i])));
+      }
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i) s += j0 + i * 32 == r.without ? 0.0 : double(weight_of(x[i]));
+    }
+  } else {
+    for (uint32_t j = j0; j < vocab; j += 32) s += r.at(j);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
 
 // Drafts of sequence b, within bounds.
 __device__ __forceinline__ uint32_t drafts_of(const VerifyArgs& a, uint32_t b) {
@@ -73,14 +109,15 @@ __device__ __forceinline__ uint32_t accepted_of(const VerifyArgs& a, uint32_t b,
   if (lane < n) {
     const int32_t x = a.tokens[uint64_t(b) * a.drafts + lane];
     if (uint32_t(x) < a.vocab) {
-      const double p = weight_of(a.p[b * a.p_ss + lane * a.p_rs + uint32_t(x)]);
-      const double q = a.q ? weight_of(a.q[b * a.q_ss + lane * a.q_rs + uint32_t(x)]) : 1.0;
-      ok = double(a.u[uint64_t(b) * a.drafts + lane]) * q < p;  // exact: 24 + 24 bits
+      const float p = weight_of(a.p[b * a.p_ss + lane * a.p_rs + uint32_t(x)]);
+      const float q = a.q ? weight_of(a.q[b * a.q_ss + lane * a.q_rs + uint32_t(x)]) : 1.f;
+      ok = double(a.u[uint64_t(b) * a.drafts + lane]) * double(q) < double(p);  // exact: 24 + 24 bits
     } else {
       atomicOr(a.err, KERR_BAD_INDEX);
     }
   }
-  return __ffs(~__ballot_sync(0xffffffffu, ok)) == 0 ? 32u : uint32_t(__ffs(~__ballot_sync(0xffffffffu, ok)) - 1);
+  const uint32_t first = __ffs(~__ballot_sync(0xffffffffu, ok));  // 1 + the first that was not accepted
+  return first ? first - 1 : 32u;
 }
 
 __device__ __forceinline__ Rest rest_of(const VerifyArgs& a, uint32_t b, uint32_t taken) {
@@ -98,51 +135,16 @@ __device__ __forceinline__ Rest rest_of(const VerifyArgs& a, uint32_t b, uint32_
 }
 
 __global__ void __launch_bounds__(kThreads) verify_sum_kernel(const __grid_constant__ VerifyArgs a) {
-  __shared__ uint32_t s_taken;
-  __shared__ double2 s_sum[kThreads / 32];
-  const uint32_t b = blockIdx.y, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const uint32_t b = blockIdx.y, lane = threadIdx.x & 31, w = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   pdl_launch_dependents();
   pdl_wait();
-  if (w == 0) {
-    const uint32_t taken = accepted_of(a, b, lane);
-    if (lane == 0) {
-      s_taken = taken;
-      if (blockIdx.x == 0) a.accepted[b] = int32_t(taken);
-    }
-  }
-  __syncthreads();
-  const Rest r = rest_of(a, b, s_taken);
-  for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-    const uint32_t j0 = c * kChunk + threadIdx.x;
-    float x[kEach], y[kEach];
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-      const uint32_t j = j0 + i * kThreads;
-      x[i] = j < a.vocab ? __ldg(r.p + j) : 0.f;
-      y[i] = r.q && j < a.vocab ? __ldg(r.q + j) : 0.f;
-    }
-    double2 s = {0.0, 0.0};
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-      const double p = weight_of(x[i]);
-      s.y += p;
-      s.x += j0 + i * kThreads == r.without ? 0.0 : fmax(p - weight_of(y[i]), 0.0);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
-      s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
-    }
-    if (lane == 0) s_sum[w] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (uint32_t i = 1; i < kThreads / 32; ++i) {
-        s.x += s_sum[i].x;
-        s.y += s_sum[i].y;
-      }
-      a.sums[uint64_t(b) * a.chunks + c] = s;
-    }
-    __syncthreads();
+  if (w >= a.chunks && w) return;
+  const uint32_t taken = accepted_of(a, b, lane);
+  if (w == 0 && lane == 0) a.accepted[b] = int32_t(taken);
+  const Rest r = rest_of(a, b, taken);
+  for (uint32_t c = w; c < a.chunks; c += gridDim.x * (kThreads / 32)) {
+    const double s = chunk_sum(r, c, a.vocab, lane);
+    if (lane == 0) a.sums[uint64_t(b) * a.chunks + c] = s;
   }
 }
 
@@ -168,6 +170,15 @@ __device__ __forceinline__ double pick_prefix(double v, double* s_w, double* tot
   return w ? before + v : v;
 }
 
+// The lowest index with weight whose end passes the goal, and the highest with
+// weight at all; index rises with the lane, one atomic a warp.
+__device__ __forceinline__ void note_borders(bool weight, bool passes, uint32_t index, uint32_t* pick, uint32_t* last) {
+  const uint32_t lane = threadIdx.x & 31, any = __ballot_sync(0xffffffffu, weight);
+  const uint32_t hit = __ballot_sync(0xffffffffu, weight && passes);
+  if (hit && lane == uint32_t(__ffs(hit) - 1)) atomicMin(pick, index);
+  if (any && lane == uint32_t(31 - __clz(any))) atomicMax(reinterpret_cast<int*>(last), int(index));
+}
+
 __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
   __shared__ double s_w[32], s_base;
   __shared__ uint32_t s_pick, s_last;
@@ -177,21 +188,28 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const __grid_
   pdl_wait();
   const uint32_t taken = uint32_t(a.accepted[b]);
   Rest r = rest_of(a, b, taken);
-  const double2* sums = a.sums + uint64_t(b) * a.chunks;
-  // totals; where the difference is nothing, the target's row itself
-  double total = 0.0, plain = 0.0, t;
-  for (uint32_t c0 = 0; c0 < a.chunks; c0 += kPickThreads) {
-    const double2 s = c0 + tid < a.chunks ? sums[c0 + tid] : make_double2(0.0, 0.0);
-    pick_prefix(s.x, s_w, &t);
+  double* sums = a.sums + uint64_t(b) * a.chunks;
+  // up to kPickThreads chunks (524,288 tokens) one scan gives total and borders
+  double first_total, t;
+  const double first = tid < a.chunks ? sums[tid] : 0.0, first_end = pick_prefix(first, s_w, &first_total);
+  double total = first_total;
+  for (uint32_t c0 = kPickThreads; c0 < a.chunks; c0 += kPickThreads) {
+    pick_prefix(c0 + tid < a.chunks ? sums[c0 + tid] : 0.0, s_w, &t);
     total += t;
-    pick_prefix(s.y, s_w, &t);
-    plain += t;
   }
-  const bool whole = !(total > 0.0);
-  if (whole) {
-    total = plain;
+  const bool again = !(total > 0.0);
+  if (again) {  // seldom: the difference is nothing; the target's row itself
     r.q = nullptr;
     r.without = 0xffffffffu;
+    for (uint32_t c = tid >> 5; c < a.chunks; c += kPickThreads / 32) {
+      const double s = chunk_sum(r, c, a.vocab, tid & 31);
+      if ((tid & 31) == 0) sums[c] = s;
+    }
+    __syncthreads();
+    for (uint32_t c0 = 0; c0 < a.chunks; c0 += kPickThreads) {
+      pick_prefix(c0 + tid < a.chunks ? sums[c0 + tid] : 0.0, s_w, &t);
+      total += t;
+    }
   }
   if (!(total > 0.0)) {
     if (tid == 0) a.next[b] = -1;
@@ -201,12 +219,13 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const __grid_
   // the first chunk whose end passes the goal; rounding may leave none: the last one with any weight
   double run = 0.0;
   for (uint32_t c0 = 0; c0 < a.chunks; c0 += kPickThreads) {
-    const double2 s = c0 + tid < a.chunks ? sums[c0 + tid] : make_double2(0.0, 0.0);
-    const double v = whole ? s.y : s.x, end = run + pick_prefix(v, s_w, &t);
-    if (v > 0.0) {
-      if (end > goal) atomicMin(&s_pick, c0 + tid);
-      atomicMax(reinterpret_cast<int*>(&s_last), int(c0 + tid));
+    double v = first, end = first_end;
+    t = first_total;
+    if (c0 || again) {
+      v = c0 + tid < a.chunks ? sums[c0 + tid] : 0.0;
+      end = run + pick_prefix(v, s_w, &t);
     }
+    note_borders(v > 0.0, end > goal, c0 + tid, &s_pick, &s_last);
     __syncthreads();
     if (s_pick == c0 + tid || (s_pick == 0xffffffffu && s_last == c0 + tid)) s_base = end - v;
     run += t;
@@ -218,29 +237,16 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const __grid_
   __syncthreads();
   if (tid == 0) s_pick = 0xffffffffu, s_last = 0xffffffffu;
   __syncthreads();
-  constexpr uint32_t kMine = kChunk / kPickThreads;  // neighbouring tokens of a thread
-  double x[kMine], sum = 0.0, unused;
-#pragma unroll
-  for (uint32_t i = 0; i < kMine; ++i) {
-    const uint32_t j = c * kChunk + tid * kMine + i;
-    x[i] = j < a.vocab ? r.at(j, &unused) : 0.0;
-    sum += x[i];
-  }
-  double end = base + (pick_prefix(sum, s_w, &t) - sum);
-#pragma unroll
-  for (uint32_t i = 0; i < kMine; ++i) {
-    end += x[i];
-    if (x[i] > 0.0) {
-      if (end > goal) atomicMin(&s_pick, c * kChunk + tid * kMine + i);
-      atomicMax(reinterpret_cast<int*>(&s_last), int(c * kChunk + tid * kMine + i));
-    }
-  }
+  static_assert(kChunk <= kPickThreads, "a thread a token");
+  const uint32_t j = c * kChunk + tid;
+  const double x = tid < kChunk && j < a.vocab ? r.at(j) : 0.0, end = base + pick_prefix(x, s_w, &t);
+  note_borders(x > 0.0, end > goal, j, &s_pick, &s_last);
   __syncthreads();
   if (tid == 0) a.next[b] = int32_t(s_pick != 0xffffffffu ? s_pick : s_last);
 }
 
 uint64_t verify_bytes(uint32_t sequences, uint32_t vocab) {
-  return uint64_t(sequences) * ((uint64_t(vocab) + kChunk - 1) / kChunk) * sizeof(double2);
+  return uint64_t(sequences) * ((uint64_t(vocab) + kChunk - 1) / kChunk) * sizeof(double);
 }
 
 int check_sizes(uint32_t sequences, uint32_t vocab, std::string* msg) {
@@ -298,10 +304,14 @@ extern "C" int si_verify_drafts_dev(si_ctx* ctx, const si_verify_drafts* a, void
   p.accepted = a->accepted, p.next = a->next;
   p.drafts = a->drafts, p.vocab = a->vocab;
   p.chunks = uint32_t((uint64_t(a->vocab) + kChunk - 1) / kChunk);
-  p.sums = static_cast<double2*>(a->work);
+  p.sums = static_cast<double*>(a->work);
   p.err = ctx->d_err;
   const cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-  PdlLaunch l(dim3(std::min(p.chunks, 65535u), a->sequences), dim3(kThreads), 0, s);
+  // CTAs for every chunk at small batches; at large ones a few a sequence, which
+  // then share the beginning (three dependent loads) among several chunks
+  const uint32_t all = (p.chunks + kThreads / 32 - 1) / (kThreads / 32);
+  const uint32_t few = std::max(1u, uint32_t(ctx->sm_count) * 16 / a->sequences);
+  PdlLaunch l(dim3(std::min(all, few), a->sequences), dim3(kThreads), 0, s);
   if (cudaError_t e = cudaLaunchKernelEx(&l.cfg, verify_sum_kernel, p)) return cuda_fail(ctx, e, "draft verification launch");
   PdlLaunch k(dim3(a->sequences), dim3(kPickThreads), 0, s);
   if (cudaError_t e = cudaLaunchKernelEx(&k.cfg, verify_pick_kernel, p)) return cuda_fail(ctx, e, "draft verification launch");
