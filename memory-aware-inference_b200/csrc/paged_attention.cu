@@ -89,14 +89,14 @@ struct AttArgs {
   int* err;
 };
 
-// 16 bytes into r if `on`, else r stays: predicated, so that loads stay in one
-// run without branches between them.
-__device__ __forceinline__ void ldg_if(uint4& r, const void* p, bool on) {
+// 16 bytes into r if index < count, else r stays: predicated, so that loads
+// stay in one run without branches between them.
+__device__ __forceinline__ void ldg_if(uint4& r, const void* p, uint32_t index, uint32_t count) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %5, %6;\n\t"
       "@p ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
       : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
-      : "l"(p), "r"(uint32_t(on)));
+      : "l"(p), "r"(index), "r"(count));
 }
 // 16 bytes to shared memory, zeros if not `on`.
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool on) {
@@ -114,6 +114,25 @@ __device__ __forceinline__ void mma16(float d[4], const uint32_t a[4], uint32_t 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The first product of a sum: nothing to add to.
+template <bool BF16>
+__device__ __forceinline__ void mma16_first(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// (x0, x1) += (y0, y1), rounded to nearest, in one instruction.
+__device__ __forceinline__ void add2(float& x0, float& x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(y0), "f"(y1));
 }
 
 // Pair (x, y) rounded to 16 bits, and what the rounding left.
@@ -272,6 +291,8 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
   float* region = smem + w * kRegion;
   uint4* s_q = reinterpret_cast<uint4*>(region) + lane;  // [step][term][lane]: a lane reads what it wrote
   const uint32_t chunks = a.kv.hd / 8;
+  // steps in which the lane has dims below head_dim
+  const uint32_t k_steps = (chunks + 3 - c4) / 4, v_steps = (chunks + 7 - n8) / 8;
 
   Place at;
   if (u0 < u1) at = place_of(u0, prefix, a.kv.sequences, heads);
@@ -318,11 +339,12 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
       const uint64_t c0 = shfl64(cell, n8), c1 = shfl64(cell, n8 + 8);
       lo = c0 != kNoCell;
       hi = c1 != kNoCell;
+      const uint16_t *p0 = a.kv.k + c0 + c4 * 8, *p1 = a.kv.k + c1 + c4 * 8;
+      const uint32_t n0 = lo ? k_steps : 0, n1 = hi ? k_steps : 0;
 #pragma unroll
-      for (int s = 0; s < KK; ++s) {
-        const uint32_t ch = 4 * s + c4;
-        ldg_if(kr[0][s], a.kv.k + c0 + ch * 8, lo && ch < chunks);
-        ldg_if(kr[1][s], a.kv.k + c1 + ch * 8, hi && ch < chunks);
+      for (uint32_t s = 0; s < KK; ++s) {
+        ldg_if(kr[0][s], p0 + s * 32, s, n0);
+        ldg_if(kr[1][s], p1 + s * 32, s, n1);
       }
     };
     auto load_v = [&](uint64_t cell) {
@@ -336,11 +358,10 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t c = shfl64(cell, 2 * c4 + (i & 1) + (i >> 1) * 8);
+        const uint16_t* p = a.kv.v + c + n8 * 8;
+        const uint32_t n = c != kNoCell ? v_steps : 0;
 #pragma unroll
-        for (int d = 0; d < KV; ++d) {
-          const uint32_t ch = 8 * d + n8;
-          ldg_if(vr[i][d], a.kv.v + c + ch * 8, c != kNoCell && ch < chunks);
-        }
+        for (uint32_t d = 0; d < KV; ++d) ldg_if(vr[i][d], p + d * 64, d, n);
       }
     };
     bool lo, hi;
@@ -413,7 +434,7 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
       const int32_t page_after = page_of(tile + 2);
       // Several chains of dependent products, two a term: shorter ones, fewer
       // roundings of a large sum, and small terms are not lost in large ones.
-      float s[4] = {}, chain[2 * TQ - 1][4] = {};
+      float s[4], chain[2 * TQ - 1][4];
 #pragma unroll
       for (int st = 0; st < KK; ++st) {
         const uint4 x = kr[0][st], y = kr[1][st];
@@ -421,8 +442,13 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
 #pragma unroll
         for (int t = 0; t < TQ; ++t) {
           const uint4 qv = s_q[(st * TQ + t) * 32];
-          mma16<BF16>(t ? chain[2 * t - 1] : s, a0, qv.x, qv.y);
-          mma16<BF16>(chain[2 * t], a1, qv.z, qv.w);
+          if (st == 0) {
+            mma16_first<BF16>(t ? chain[2 * t - 1] : s, a0, qv.x, qv.y);
+            mma16_first<BF16>(chain[2 * t], a1, qv.z, qv.w);
+          } else {
+            mma16<BF16>(t ? chain[2 * t - 1] : s, a0, qv.x, qv.y);
+            mma16<BF16>(chain[2 * t], a1, qv.z, qv.w);
+          }
         }
       }
 #pragma unroll
@@ -493,11 +519,12 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
           if constexpr (TQ > 1) {
             // The tensor core cuts its sums off: the unit's products are summed
             // by themselves and added, rounded, to the running sum.
-            float o[4] = {};
+            float o[4];
+            mma16_first<BF16>(o, av, pb[TP - 1][0], pb[TP - 1][1]);
 #pragma unroll
-            for (int t = TP - 1; t >= 0; --t) mma16<BF16>(o, av, pb[t][0], pb[t][1]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[d * 4 + j][i] += o[i];
+            for (int t = TP - 2; t >= 0; --t) mma16<BF16>(o, av, pb[t][0], pb[t][1]);
+            add2(acc[d * 4 + j][0], acc[d * 4 + j][1], o[0], o[1]);
+            add2(acc[d * 4 + j][2], acc[d * 4 + j][3], o[2], o[3]);
           } else {
 #pragma unroll
             for (int t = TP - 1; t >= 0; --t) mma16<BF16>(acc[d * 4 + j], av, pb[t][0], pb[t][1]);
