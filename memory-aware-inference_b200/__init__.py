@@ -813,9 +813,8 @@ class CudaContext:
     # -- paged cache (include/si_paged.h; descriptions from paged.py) ---------
     def _here(self, described):
         """Refuses a description whose tensors are not on this context's GPU."""
-        held = getattr(described, "_tensors", None)
-        if held and (held[0].device.type != "cuda" or held[0].device.index != self.device):
-            raise SiError(SI_E_INVALID, f"tensors are on {held[0].device}, the context on cuda:{self.device}")
+        if getattr(described, "_device", self.device) != self.device:
+            raise SiError(SI_E_INVALID, f"tensors are on {described._tensors[0].device}, the context on cuda:{self.device}")
 
     def paged_append_dev(self, kv: SiPagedKv, append: SiPagedAppend, stream=None):
         """si_paged_append_dev: rotary positions of new queries and keys, keys and values into pages."""

@@ -648,11 +648,13 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
 
 // Joins the partials of the pairs that cross CTA borders. Block (i, column):
 // the pair whose first border is the one before CTA i + 1, one query head of
-// it. A pair may lie in as many partials as there are CTAs; four groups of
-// threads take every fourth each, in batches whose loads are all in flight.
-constexpr int kJoinGroups = 4, kJoinBatch = 10;
+// it. A pair may lie in as many partials as there are CTAs: a batch's loads are
+// all in flight. Most blocks find nothing to join, so the blocks are small and
+// all resident at once (1024 threads a block took 3 us longer at 147 x 6 blocks).
+constexpr int kJoinBatch = 16;
 template <int HD>
-__global__ void __launch_bounds__(HD * kJoinGroups) paged_join_kernel(const __grid_constant__ AttArgs a, float shift) {
+__global__ void __launch_bounds__(HD >= 192 ? HD : 256) paged_join_kernel(const __grid_constant__ AttArgs a, float shift) {
+  constexpr int kJoinGroups = HD >= 192 ? 1 : 256 / HD;
   constexpr uint32_t kPart = kCols * (HD + 2);
   __shared__ float s_o[kJoinGroups][HD], s_m[kJoinGroups], s_l[kJoinGroups];
   pdl_launch_dependents();
@@ -816,7 +818,7 @@ cudaError_t launch(const AttArgs& p, uint32_t grid, cudaStream_t s) {
   PdlLaunch l(dim3(grid), dim3(Shape<HD>::kWarps * 32), smem, s);
   if (cudaError_t e = cudaLaunchKernelEx(&l.cfg, kernel, p)) return e;
   if (grid == 1) return cudaSuccess;
-  PdlLaunch j(dim3(grid - 1, std::min(kCols, p.group)), dim3(HD * kJoinGroups), 0, s);
+  PdlLaunch j(dim3(grid - 1, std::min(kCols, p.group)), dim3(HD >= 192 ? HD : 256), 0, s);
   return cudaLaunchKernelEx(&j.cfg, paged_join_kernel<HD>, p, BF16 ? 0.f : 15.f);
 }
 

@@ -22,6 +22,8 @@ class _Described(C.Structure):
 
     def _hold(self, *tensors):
         self._tensors = [t for t in tensors if t is not None]
+        at = self._tensors[0].device
+        self._device = at.index if at.type == "cuda" else -1
         return self
 
 
