@@ -11,13 +11,12 @@
 // formed and summed in f64; two sums of different order differ by 1e-16, so
 // they choose differently about once in 10^10 draws.
 //
-// Two kernels. Every warp of the first decides the sequence's accepted count
-// for itself (a few loads) and sums chunks of 512 tokens of the row, no barrier;
-// one CTA a sequence of the second scans the chunk sums, finds the chunk that
-// the draw falls in, and scans that chunk. The row is read once, one chunk of
-// it twice. A difference is max(p - q, 0) = p - min(p, q), so that the minimum is
-// taken in f32 and only the subtraction and the sum in f64: conversions have an eighth
-// of the f32 rate and were what bound the sums at first.
+// One kernel: a cluster of 1 to 8 CTAs a sequence. Every warp decides the
+// accepted count for itself (a few loads, no barrier) and sums its own run of
+// the row's tokens; the CTAs' totals meet over distributed shared memory, every CTA
+// finds whose run the draw falls in, and that CTA scans that warp's run
+// again. A difference is max(p - q, 0) = p - min(p, q), so that the minimum is
+// taken in f32 and only the subtraction and the sum in f64.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -27,8 +26,8 @@
 namespace si {
 namespace {
 
-constexpr uint32_t kThreads = 256, kEach = 16, kChunk = 32 * kEach;  // tokens of a chunk
-constexpr uint32_t kPickThreads = 1024;
+constexpr uint32_t kEach = 16, kTurn = 32 * kEach;  // tokens of a warp and turn
+constexpr uint32_t kMaxCluster = 8;
 
 struct VerifyArgs {
   const float *p, *q;
@@ -36,8 +35,7 @@ struct VerifyArgs {
   const int32_t *tokens, *counts;
   const float *u, *u_last;
   int32_t *accepted, *next;
-  uint32_t drafts, vocab, chunks;
-  double* sums;  // [sequence][chunk]
+  uint32_t drafts, vocab;
   int* err;
 };
 
@@ -62,18 +60,18 @@ __device__ __forceinline__ float load_stream(const float* p) {
   return x;
 }
 
-// Sum of chunk c by one warp, the same in all lanes. All loads are on their way
-// before the first value is used.
-__device__ __forceinline__ double chunk_sum(const Rest& r, uint32_t c, uint32_t vocab, uint32_t lane) {
-  const uint32_t j0 = c * kChunk + lane;
+// Sum of tokens [j0, j1) by one warp, the same in all lanes. All loads of a turn
+// are on their way before the first value is used.
+__device__ __forceinline__ double run_sum(const Rest& r, uint32_t j0, uint32_t j1, uint32_t lane) {
   double s = 0.0;
-  float x[kEach], y[kEach];
-  if (c * kChunk + kChunk <= vocab) {
+  uint32_t j = j0 + lane;
+  for (; j - lane + kTurn <= j1; j += kTurn) {
+    float x[kEach], y[kEach];
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) x[i] = load_stream(r.p + j0 + i * 32);
+    for (uint32_t i = 0; i < kEach; ++i) x[i] = load_stream(r.p + j + i * 32);
     if (r.q) {
 #pragma unroll
-      for (uint32_t i = 0; i < kEach; ++i) y[i] = load_stream(r.q + j0 + i * 32);
+      for (uint32_t i = 0; i < kEach; ++i) y[i] = load_stream(r.q + j + i * 32);
 #pragma unroll
       for (uint32_t i = 0; i < kEach; ++i) {
         const float w = weight_of(x[i]);
@@ -81,11 +79,11 @@ __device__ __forceinline__ double chunk_sum(const Rest& r, uint32_t c, uint32_t 
       }
     } else {
 #pragma unroll
-      for (uint32_t i = 0; i < kEach; ++i) s += j0 + i * 32 == r.without ? 0.0 : double(weight_of(x[i]));
+      for (uint32_t i = 0; i < kEach; ++i) s += j + i * 32 == r.without ? 0.0 : double(weight_of(x[i]));
     }
-  } else {
-    for (uint32_t j = j0; j < vocab; j += 32) s += r.at(j);
   }
+#pragma unroll 4
+  for (; j < j1; j += 32) s += r.at(j);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
@@ -134,40 +132,42 @@ __device__ __forceinline__ Rest rest_of(const VerifyArgs& a, uint32_t b, uint32_
   return r;
 }
 
-__global__ void __launch_bounds__(kThreads) verify_sum_kernel(const __grid_constant__ VerifyArgs a) {
-  const uint32_t b = blockIdx.y, lane = threadIdx.x & 31, w = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  pdl_launch_dependents();
-  pdl_wait();
-  if (w >= a.chunks && w) return;
-  const uint32_t taken = accepted_of(a, b, lane);
-  if (w == 0 && lane == 0) a.accepted[b] = int32_t(taken);
-  const Rest r = rest_of(a, b, taken);
-  for (uint32_t c = w; c < a.chunks; c += gridDim.x * (kThreads / 32)) {
-    const double s = chunk_sum(r, c, a.vocab, lane);
-    if (lane == 0) a.sums[uint64_t(b) * a.chunks + c] = s;
-  }
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ double peer_f64(const double* p, uint32_t rank) {
+  uint32_t at;
+  double v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
+  return v;
 }
 
-// Inclusive prefix of one value a thread over kPickThreads threads.
-__device__ __forceinline__ double pick_prefix(double v, double* s_w, double* total) {
-  const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+// Inclusive prefix over the lanes.
+__device__ __forceinline__ double lane_prefix(double v, uint32_t lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const double y = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= uint32_t(o)) v += y;
   }
-  __syncthreads();
-  if (lane == 31) s_w[w] = v;
-  __syncthreads();
-  double y = s_w[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double z = __shfl_up_sync(0xffffffffu, y, o);
-    if (lane >= uint32_t(o)) y += z;
-  }
-  *total = __shfl_sync(0xffffffffu, y, 31);
-  const double before = __shfl_sync(0xffffffffu, y, w ? w - 1 : 0);
-  return w ? before + v : v;
+  return v;
+}
+// Of lanes in order, each with a weight and the end of its share of the line:
+// the first with weight whose end passes the goal; rounding may leave none:
+// the last one with any weight. 32: no weight at all.
+__device__ __forceinline__ uint32_t pick_lane(double weight, double end, double goal) {
+  const uint32_t any = __ballot_sync(0xffffffffu, weight > 0.0);
+  const uint32_t hit = __ballot_sync(0xffffffffu, weight > 0.0 && end > goal);
+  return hit ? __ffs(hit) - 1 : any ? 31 - __clz(any) : 32;
 }
 
 // The lowest index with weight whose end passes the goal, and the highest with
@@ -179,75 +179,80 @@ __device__ __forceinline__ void note_borders(bool weight, bool passes, uint32_t 
   if (any && lane == uint32_t(31 - __clz(any))) atomicMax(reinterpret_cast<int*>(last), int(index));
 }
 
-__global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
-  __shared__ double s_w[32], s_base;
+template <uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const __grid_constant__ VerifyArgs a) {
+  constexpr uint32_t kWarps = THREADS / 32;
+  __shared__ double s_run[kWarps], s_total, s_scan[kWarps];
   __shared__ uint32_t s_pick, s_last;
-  const uint32_t b = blockIdx.x, tid = threadIdx.x;
-  if (tid == 0) s_pick = 0xffffffffu, s_last = 0xffffffffu, s_base = 0.0;
+  const uint32_t rank = cluster_rank(), size = cluster_size(), b = blockIdx.x / size;
+  const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t taken = uint32_t(a.accepted[b]);
+  const uint32_t taken = accepted_of(a, b, lane);
+  if (rank == 0 && threadIdx.x == 0) a.accepted[b] = int32_t(taken);
   Rest r = rest_of(a, b, taken);
-  double* sums = a.sums + uint64_t(b) * a.chunks;
-  // up to kPickThreads chunks (524,288 tokens) one scan gives total and borders
-  double first_total, t;
-  const double first = tid < a.chunks ? sums[tid] : 0.0, first_end = pick_prefix(first, s_w, &first_total);
-  double total = first_total;
-  for (uint32_t c0 = kPickThreads; c0 < a.chunks; c0 += kPickThreads) {
-    pick_prefix(c0 + tid < a.chunks ? sums[c0 + tid] : 0.0, s_w, &t);
-    total += t;
-  }
-  const bool again = !(total > 0.0);
-  if (again) {  // seldom: the difference is nothing; the target's row itself
-    r.q = nullptr;
-    r.without = 0xffffffffu;
-    for (uint32_t c = tid >> 5; c < a.chunks; c += kPickThreads / 32) {
-      const double s = chunk_sum(r, c, a.vocab, tid & 31);
-      if ((tid & 31) == 0) sums[c] = s;
+  // runs of whole turns, but for the row's end
+  const uint32_t turns = (a.vocab + kTurn - 1) / kTurn, runs = size * kWarps;
+  auto border = [&](uint32_t i) { return uint32_t(min(uint64_t(a.vocab), uint64_t(turns) * i / runs * kTurn)); };
+  double total = 0.0, mine = 0.0, before = 0.0;  // cluster's sum, this warp's, those of the CTAs before
+  uint32_t owner = size;                           // the CTA that the draw falls in
+  double goal = 0.0;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    if (attempt) {  // seldom: the difference is nothing; the target's row itself
+      r.q = nullptr;
+      r.without = 0xffffffffu;
     }
+    const uint32_t i = rank * kWarps + w;
+    mine = run_sum(r, border(i), border(i + 1), lane);
+    if (lane == 0) s_run[w] = mine;
     __syncthreads();
-    for (uint32_t c0 = 0; c0 < a.chunks; c0 += kPickThreads) {
-      pick_prefix(c0 + tid < a.chunks ? sums[c0 + tid] : 0.0, s_w, &t);
-      total += t;
+    if (w == 0) {
+      const double t = lane_prefix(lane < kWarps ? s_run[lane] : 0.0, lane);
+      if (lane == 31) s_total = t;
     }
+    cluster_arrive();
+    cluster_wait();
+    const double share = lane < size ? peer_f64(&s_total, lane) : 0.0;
+    const double end = lane_prefix(share, lane);
+    total = __shfl_sync(0xffffffffu, end, 31);
+    goal = double(a.u_last[b]) * total;
+    owner = pick_lane(share, end, goal);
+    before = __shfl_sync(0xffffffffu, end - share, owner & 31);
+    cluster_arrive();  // this CTA has read the totals
+    if (total > 0.0 || attempt) break;  // the same decision in all CTAs
+    cluster_wait();
   }
-  if (!(total > 0.0)) {
-    if (tid == 0) a.next[b] = -1;
+  // A CTA may not leave, nor its totals change, before all have read them.
+  if (!(total > 0.0) || rank != owner) {
+    if (!(total > 0.0) && rank == 0 && threadIdx.x == 0) a.next[b] = -1;
+    cluster_wait();
     return;
   }
-  const double goal = double(a.u_last[b]) * total;
-  // the first chunk whose end passes the goal; rounding may leave none: the last one with any weight
-  double run = 0.0;
-  for (uint32_t c0 = 0; c0 < a.chunks; c0 += kPickThreads) {
-    double v = first, end = first_end;
-    t = first_total;
-    if (c0 || again) {
-      v = c0 + tid < a.chunks ? sums[c0 + tid] : 0.0;
-      end = run + pick_prefix(v, s_w, &t);
-    }
-    note_borders(v > 0.0, end > goal, c0 + tid, &s_pick, &s_last);
+  // the warp's run within the CTA, found by every warp alike
+  const double run = lane < kWarps ? s_run[lane] : 0.0, run_end = before + lane_prefix(run, lane);
+  const uint32_t at = pick_lane(run, run_end, goal);
+  double base = __shfl_sync(0xffffffffu, run_end - run, at & 31);
+  const uint32_t j0 = border(rank * kWarps + at), j1 = border(rank * kWarps + at + 1);
+  if (threadIdx.x == 0) s_pick = 0xffffffffu, s_last = 0xffffffffu;
+  for (uint32_t j = j0; j < j1; j += THREADS) {  // a token a thread
+    const uint32_t t = j + threadIdx.x;
+    const double x = t < j1 ? r.at(t) : 0.0, in_warp = lane_prefix(x, lane);
     __syncthreads();
-    if (s_pick == c0 + tid || (s_pick == 0xffffffffu && s_last == c0 + tid)) s_base = end - v;
-    run += t;
+    if (lane == 31) s_scan[w] = in_warp;
+    __syncthreads();
+    const double ends = lane_prefix(lane < kWarps ? s_scan[lane] : 0.0, lane);
+    const double end = base + (w ? __shfl_sync(0xffffffffu, ends, (w + 31) & 31) : 0.0) + in_warp;
+    note_borders(x > 0.0, end > goal, t, &s_pick, &s_last);
+    base += __shfl_sync(0xffffffffu, ends, 31);
+    __syncthreads();
     if (s_pick != 0xffffffffu) break;  // the same for all threads
   }
-  __syncthreads();
-  const uint32_t c = s_pick != 0xffffffffu ? s_pick : s_last;
-  const double base = s_base;
-  __syncthreads();
-  if (tid == 0) s_pick = 0xffffffffu, s_last = 0xffffffffu;
-  __syncthreads();
-  static_assert(kChunk <= kPickThreads, "a thread a token");
-  const uint32_t j = c * kChunk + tid;
-  const double x = tid < kChunk && j < a.vocab ? r.at(j) : 0.0, end = base + pick_prefix(x, s_w, &t);
-  note_borders(x > 0.0, end > goal, j, &s_pick, &s_last);
-  __syncthreads();
-  if (tid == 0) a.next[b] = int32_t(s_pick != 0xffffffffu ? s_pick : s_last);
+  if (threadIdx.x == 0) a.next[b] = int32_t(s_pick != 0xffffffffu ? s_pick : s_last);
+  cluster_wait();
 }
 
-uint64_t verify_bytes(uint32_t sequences, uint32_t vocab) {
-  return uint64_t(sequences) * ((uint64_t(vocab) + kChunk - 1) / kChunk) * sizeof(double);
-}
+// Nothing is kept between CTAs in memory; the smallest workspace that a caller can hold.
+uint64_t verify_bytes() { return 16; }
 
 int check_sizes(uint32_t sequences, uint32_t vocab, std::string* msg) {
   if (sequences == 0 || sequences > 65535 || vocab == 0 || vocab > 0x7fffffffu) {
@@ -270,7 +275,7 @@ int check_verify(const si_verify_drafts* a, std::string* msg) {
   if (a->drafts && (!a->tokens || !a->uniform)) return bad(SI_E_INVALID, "draft verification has no drafts or random numbers");
   for (uint64_t s : {a->target_seq_stride, a->target_row_stride, a->draft_seq_stride, a->draft_row_stride})
     if (s >> 44) return bad(SI_E_INVALID, "draft verification strides are out of range");
-  const uint64_t need = verify_bytes(a->sequences, a->vocab);
+  const uint64_t need = verify_bytes();
   if (!a->work || reinterpret_cast<uintptr_t>(a->work) % 16 || a->work_bytes < need)
     return bad(SI_E_INVALID, "draft verification needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
   return SI_OK;
@@ -285,7 +290,7 @@ extern "C" int si_verify_drafts_workspace(uint32_t sequences, uint32_t vocab, ui
   std::string msg;
   if (int rc = check_sizes(sequences, vocab, &msg)) return fail(nullptr, rc, msg);
   if (!bytes) return fail(nullptr, SI_E_INVALID, "null workspace size");
-  *bytes = verify_bytes(sequences, vocab);
+  *bytes = verify_bytes();
   return SI_OK;
 }
 
@@ -303,18 +308,20 @@ extern "C" int si_verify_drafts_dev(si_ctx* ctx, const si_verify_drafts* a, void
   p.u = a->uniform, p.u_last = a->last_uniform;
   p.accepted = a->accepted, p.next = a->next;
   p.drafts = a->drafts, p.vocab = a->vocab;
-  p.chunks = uint32_t((uint64_t(a->vocab) + kChunk - 1) / kChunk);
-  p.sums = static_cast<double*>(a->work);
   p.err = ctx->d_err;
   const cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-  // CTAs for every chunk at small batches; at large ones a few a sequence, which
-  // then share the beginning (three dependent loads) among several chunks
-  const uint32_t all = (p.chunks + kThreads / 32 - 1) / (kThreads / 32);
-  const uint32_t few = std::max(1u, uint32_t(ctx->sm_count) * 16 / a->sequences);
-  PdlLaunch l(dim3(std::min(all, few), a->sequences), dim3(kThreads), 0, s);
-  if (cudaError_t e = cudaLaunchKernelEx(&l.cfg, verify_sum_kernel, p)) return cuda_fail(ctx, e, "draft verification launch");
-  PdlLaunch k(dim3(a->sequences), dim3(kPickThreads), 0, s);
-  if (cudaError_t e = cudaLaunchKernelEx(&k.cfg, verify_pick_kernel, p)) return cuda_fail(ctx, e, "draft verification launch");
+  // A CTA of 1024 threads a multiprocessor, or two of 512 where the sequences fill
+  // those: as many a sequence as run at once, and as the row has runs for.
+  const uint32_t sms = uint32_t(ctx->sm_count);
+  const bool large = a->sequences * 2 > sms;
+  const uint32_t turns = (a->vocab + kTurn - 1) / kTurn, warps = large ? 16 : 32;
+  uint32_t cluster = 1;
+  while (cluster < kMaxCluster && a->sequences * cluster * 2 <= (large ? 2 * sms : sms) && turns > cluster * warps)
+    cluster *= 2;
+  PdlLaunch l(dim3(a->sequences * cluster), dim3(warps * 32), 0, s);
+  l.cluster(cluster);
+  if (cudaError_t e = large ? cudaLaunchKernelEx(&l.cfg, verify_kernel<512>, p) : cudaLaunchKernelEx(&l.cfg, verify_kernel<1024>, p))
+    return cuda_fail(ctx, e, "draft verification launch");
   note_async_submission(ctx);
   return SI_OK;
 }
