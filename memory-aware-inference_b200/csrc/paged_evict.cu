@@ -44,6 +44,7 @@ struct EvictArgs {
   uint32_t budget, sink, recent;
   uint32_t most;  // longest length that the page table and the weights' rows have room for
   uint32_t room;  // entries of a move list
+  bool at_once;   // the selecting CTA moves the pairs itself
   uint32_t* moves;   // [sequence * kv_heads + head][2][room]: from, to
   uint32_t* counts;  // [sequence * kv_heads + head]
   int* err;
@@ -121,6 +122,55 @@ __device__ __forceinline__ uint32_t cta_prefix(uint32_t v, uint32_t* s_w, uint32
   }
   *total = __shfl_sync(0xffffffffu, y, 31);
   return __shfl_sync(0xffffffffu, y - mine, w) + x - v;
+}
+
+// Kept slots from behind the new length into the holes below it: sources and
+// destinations do not meet, so the order is free. Eight lanes move a pair, each
+// up to four 16-byte pieces of its key and of its value, all in flight at once.
+// Thread `thread` of `threads` (a multiple of 8).
+constexpr uint32_t kLanes = 8;
+__device__ __forceinline__ void move_pairs(const EvictArgs& a, uint32_t row, uint32_t b, uint32_t h, uint32_t pairs,
+                                           uint32_t thread, uint32_t threads) {
+  const uint32_t chunks = a.kv.hd / 8, l = thread % kLanes;
+  const uint64_t base = uint64_t(row) * a.stride;
+  const uint32_t *froms = a.moves + uint64_t(row) * 2 * a.room, *tos = froms + a.room;
+  const int32_t* pages = a.kv.pages + b * a.kv.pages_stride;
+  uint16_t *k_pool = const_cast<uint16_t*>(a.kv.k), *v_pool = const_cast<uint16_t*>(a.kv.v);
+  for (uint32_t i = thread / kLanes; i < pairs; i += threads / kLanes) {
+    const uint2 mv = make_uint2(froms[i], tos[i]);
+    const uint64_t from = paged_slot(a.kv, pages, mv.x, h), to = paged_slot(a.kv, pages, mv.y, h);
+    float w = 0.f;
+    int32_t p = 0;
+    if (l == 0) {
+      w = a.w_in[base + mv.x];
+      p = a.p_in ? a.p_in[base + mv.x] : int32_t(mv.x);
+    }
+    if (from != kNoCell && to != kNoCell) {
+      uint4 k[4], v[4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t ch = l + j * kLanes;
+        if (ch < chunks) {
+          k[j] = *reinterpret_cast<const uint4*>(k_pool + from + ch * 8);
+          v[j] = *reinterpret_cast<const uint4*>(v_pool + from + ch * 8);
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t ch = l + j * kLanes;
+        if (ch < chunks) {
+          *reinterpret_cast<uint4*>(k_pool + to + ch * 8) = k[j];
+          *reinterpret_cast<uint4*>(v_pool + to + ch * 8) = v[j];
+        }
+      }
+    } else if (l == 0) {
+      atomicOr(a.err, KERR_BAD_INDEX);
+    }
+    if (l == 0) {
+      a.w_out[base + mv.y] = w;
+      if (a.p_out) a.p_out[base + mv.y] = p;
+    }
+  }
 }
 
 template <int THREADS, bool CLUSTER>
@@ -295,13 +345,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) evict_select
     });
   }
   if (rank == 0 && tid == 0) a.counts[row] = moved;
+  if (!CLUSTER && a.at_once) {
+    __syncthreads();  // the lists, and the weights and positions that went out as they were
+    move_pairs(a, row, b, row - b * a.kv.kv_heads, moved, tid, THREADS);
+  }
   if constexpr (CLUSTER) group_sync<CLUSTER>();  // no CTA leaves while another may still read its counts
 }
 
-// Kept slots from behind the new length into the holes below it: sources and
-// destinations do not meet, so the order is free. Eight lanes move a pair, each
-// up to four 16-byte pieces of its key and of its value, all in flight at once.
-constexpr uint32_t kLanes = 8;
 __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ EvictArgs a) {
   const uint32_t row = blockIdx.y, b = row / a.kv.kv_heads, h = row - b * a.kv.kv_heads;
   pdl_launch_dependents();
@@ -310,46 +360,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__
     const int32_t n = a.len_in[b];  // read and written by this thread alone
     a.len_out[b] = int32_t(min(n < 0 ? 0u : min(uint32_t(n), a.most), a.budget));
   }
-  const uint32_t pairs = a.counts[row], chunks = a.kv.hd / 8, l = threadIdx.x % kLanes;
-  const uint64_t base = uint64_t(row) * a.stride;
-  const uint32_t *froms = a.moves + uint64_t(row) * 2 * a.room, *tos = froms + a.room;
-  const int32_t* pages = a.kv.pages + b * a.kv.pages_stride;
-  uint16_t *k_pool = const_cast<uint16_t*>(a.kv.k), *v_pool = const_cast<uint16_t*>(a.kv.v);
-  for (uint32_t i = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes; i < pairs; i += gridDim.x * (256 / kLanes)) {
-    const uint2 mv = make_uint2(froms[i], tos[i]);
-    const uint64_t from = paged_slot(a.kv, pages, mv.x, h), to = paged_slot(a.kv, pages, mv.y, h);
-    float w = 0.f;
-    int32_t p = 0;
-    if (l == 0) {
-      w = a.w_in[base + mv.x];
-      p = a.p_in ? a.p_in[base + mv.x] : int32_t(mv.x);
-    }
-    if (from != kNoCell && to != kNoCell) {
-      uint4 k[4], v[4];
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) {
-        const uint32_t ch = l + j * kLanes;
-        if (ch < chunks) {
-          k[j] = *reinterpret_cast<const uint4*>(k_pool + from + ch * 8);
-          v[j] = *reinterpret_cast<const uint4*>(v_pool + from + ch * 8);
-        }
-      }
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) {
-        const uint32_t ch = l + j * kLanes;
-        if (ch < chunks) {
-          *reinterpret_cast<uint4*>(k_pool + to + ch * 8) = k[j];
-          *reinterpret_cast<uint4*>(v_pool + to + ch * 8) = v[j];
-        }
-      }
-    } else if (l == 0) {
-      atomicOr(a.err, KERR_BAD_INDEX);
-    }
-    if (l == 0) {
-      a.w_out[base + mv.y] = w;
-      if (a.p_out) a.p_out[base + mv.y] = p;
-    }
-  }
+  move_pairs(a, row, b, h, a.counts[row], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 uint64_t rows_of(const si_paged_kv& kv) { return uint64_t(kv.sequences) * kv.kv_heads; }
@@ -445,15 +456,23 @@ extern "C" int si_paged_evict_dev(si_ctx* ctx, const si_paged_kv* kv, const si_p
          (most > cluster * kCtaSlots || rows <= (cluster == 1 ? 56u : cluster == 2 ? 24u : 8u)))
     cluster *= 2;
   const uint32_t each = (most + cluster - 1) / cluster;
+  // Moves of one row are at most the smaller of both sides of the budget. A few
+  // (a page's worth leaves in steady state) the selecting CTA makes itself, which saves a
+  // launch: 32 x 8 rows of 4,160 slots that lose 64 take 16.9 us, and 19.5 us with a second
+  // kernel. Not where the new lengths go over the old ones: other heads' CTAs
+  // still read those.
+  const uint64_t most_moves = std::min<uint64_t>(most > a->budget ? most - a->budget : 0, a->budget);
+  p.at_once = cluster == 1 && most_moves <= 256 && p.len_in != p.len_out;
   // 256, 512 or 1024 threads for about 16 keys a thread
   const cudaError_t e = cluster > 1 ? (each > 8192 ? select<1024, true>(p, rows, cluster, each, s) : select<512, true>(p, rows, cluster, each, s))
                         : each > 8192 ? select<1024, false>(p, rows, 1, each, s) : each > 2048 ? select<512, false>(p, rows, 1, each, s) : select<256, false>(p, rows, 1, each, s);
   if (e != cudaSuccess) return cuda_fail(ctx, e, "paged eviction launch");
-  // moves of one row are at most the smaller of both sides of the budget
-  const uint64_t lanes = std::min<uint64_t>(most > a->budget ? most - a->budget : 0, a->budget) * kLanes;
-  const uint32_t wide = std::max(1u, uint32_t(ctx->sm_count) * 16 / rows);
-  PdlLaunch v(dim3(uint32_t(std::max<uint64_t>(1, std::min<uint64_t>((lanes + 255) / 256, wide))), rows), dim3(256), 0, s);
-  if (cudaError_t e = cudaLaunchKernelEx(&v.cfg, evict_move_kernel, p)) return cuda_fail(ctx, e, "paged eviction launch");
+  if (!p.at_once) {
+    const uint64_t lanes = most_moves * kLanes;
+    const uint32_t wide = std::max(1u, uint32_t(ctx->sm_count) * 16 / rows);
+    PdlLaunch v(dim3(uint32_t(std::max<uint64_t>(1, std::min<uint64_t>((lanes + 255) / 256, wide))), rows), dim3(256), 0, s);
+    if (cudaError_t e = cudaLaunchKernelEx(&v.cfg, evict_move_kernel, p)) return cuda_fail(ctx, e, "paged eviction launch");
+  }
   note_async_submission(ctx);
   return SI_OK;
 }
