@@ -38,8 +38,8 @@
 // the cache's own type are exact in one term. f32 queries take 3 bf16 terms
 // (24 bits) or 2 f16 terms (22 bits, after scaling each query by a power of two
 // to a maximum near 2^15), probabilities 3 bf16 or 2 f16 terms with f32 output and
-// 2 with 16-bit output. In f16, probabilities are scaled by 2^15 so that small ones keep
-// their bits; the sum is taken of the same scaled values.
+// 2 with 16-bit output. In f16, probabilities are scaled up so that small ones keep their
+// bits; the sum is taken of the same scaled values.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -57,6 +57,10 @@ constexpr uint32_t kCols = 8;   // query heads of a block
 constexpr uint32_t kPairCost = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// Probabilities are 2^(score - reference + shift), below 2^(shift + slack): in
+// f16 as high as its range allows.
+constexpr float kSlack = 4.f;
+constexpr float shift_of(bool bf16) { return bf16 ? 0.f : 11.f; }
 
 template <int HD>
 struct Shape {
@@ -151,6 +155,13 @@ __device__ __forceinline__ uint32_t take_term(float& x, float& y) {
     y -= f.y;
     return *reinterpret_cast<const uint32_t*>(&r);
   }
+}
+
+// 2^x, zero far below; two units in the last place.
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
@@ -250,7 +261,7 @@ __device__ __forceinline__ void finish(const AttArgs& a, const Place& at, uint32
 template <int HD, bool BF16, int TQ, int TP>
 __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_kernel(const __grid_constant__ AttArgs a) {
   constexpr int NW = Shape<HD>::kWarps, KK = Shape<HD>::kK, KV = Shape<HD>::kV;
-  constexpr float kShift = BF16 ? 0.f : 15.f;
+  constexpr float kShift = shift_of(BF16);
   constexpr uint32_t kPart = kCols * (HD + 2);                   // floats of a partial: values, then max and sum
   constexpr uint32_t kQ = uint32_t(TQ * KK) * 32 * 4;            // floats of a warp's query terms
   constexpr uint32_t kRegion = (kQ > kPart ? kQ : kPart) + kPart;
@@ -475,13 +486,16 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
             *reinterpret_cast<float2*>(to + uint64_t(n8 + 8) * a.gpad) = make_float2(s[2], s[3]);
         }
       }
+      // The reference point of the exponents follows the maximum only when a score
+      // passes it by more than kSlack: that is seldom after the first units, and
+      // a vote is cheaper than the maximum over the lanes.
       float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+      if (__any_sync(0xffffffffu, x0 > m0 + kSlack || x1 > m1 + kSlack)) {
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
-      }
-      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {  // the running maximum moves seldom after the first units
+        for (int o = 4; o < 32; o <<= 1) {
+          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
+          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
+        }
         const float g0 = fmaxf(m0, x0), g1 = fmaxf(m1, x1);
         const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - g0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - g1);
         m0 = g0;
@@ -497,7 +511,7 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
         }
       }
       const float b0 = m0 == -INFINITY ? 0.f : m0 - kShift, b1 = m1 == -INFINITY ? 0.f : m1 - kShift;
-      float p[4] = {exp2f(s[0] - b0), exp2f(s[1] - b1), exp2f(s[2] - b0), exp2f(s[3] - b1)};
+      float p[4] = {pow2(s[0] - b0), pow2(s[1] - b1), pow2(s[2] - b0), pow2(s[3] - b1)};
       l0 += p[0] + p[2];
       l1 += p[1] + p[3];
       uint32_t pb[TP][2];
@@ -819,7 +833,7 @@ cudaError_t launch(const AttArgs& p, uint32_t grid, cudaStream_t s) {
   if (cudaError_t e = cudaLaunchKernelEx(&l.cfg, kernel, p)) return e;
   if (grid == 1) return cudaSuccess;
   PdlLaunch j(dim3(grid - 1, std::min(kCols, p.group)), dim3(HD >= 192 ? HD : 256), 0, s);
-  return cudaLaunchKernelEx(&j.cfg, paged_join_kernel<HD>, p, BF16 ? 0.f : 15.f);
+  return cudaLaunchKernelEx(&j.cfg, paged_join_kernel<HD>, p, shift_of(BF16));
 }
 
 template <int HD>
