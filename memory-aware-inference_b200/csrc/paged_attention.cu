@@ -358,27 +358,34 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
         ldg_if(kr[1][s], p1 + s * 32, s, n1);
       }
     };
-    auto load_v = [&](uint64_t cell) {
-      // slots that do not exist meet probability 0, and need a finite value
-      if (__any_sync(0xffffffffu, cell == kNoCell)) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int d = 0; d < KV; ++d) vr[i][d] = make_uint4(0, 0, 0, 0);
-      }
+    // A step's registers of the values are asked for again as soon as the step has used them.
+    const uint16_t* vp[4];
+    uint32_t vn[4];
+    bool v_gap = false;
+    auto rows_v = [&](uint64_t cell) {
+      v_gap = __any_sync(0xffffffffu, cell == kNoCell);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t c = shfl64(cell, 2 * c4 + (i & 1) + (i >> 1) * 8);
-        const uint16_t* p = a.kv.v + c + n8 * 8;
-        const uint32_t n = c != kNoCell ? v_steps : 0;
-#pragma unroll
-        for (uint32_t d = 0; d < KV; ++d) ldg_if(vr[i][d], p + d * 64, d, n);
+        vp[i] = a.kv.v + c + n8 * 8;
+        vn[i] = c != kNoCell ? v_steps : 0;
       }
+    };
+    auto load_v = [&](uint32_t d) {
+      // slots that do not exist meet probability 0, and need a finite value
+      if (v_gap) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vr[i][d] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ldg_if(vr[i][d], vp[i] + d * 64, d, vn[i]);
     };
     bool lo, hi;
     uint64_t cell = cell_of(t_begin, page_first);
     load_k(cell, lo, hi);
-    load_v(cell);
+    rows_v(cell);
+#pragma unroll
+    for (uint32_t d = 0; d < KV; ++d) load_v(d);
     // queries into 16-bit terms, in place; columns past the group are zero
     auto raw = [&](uint32_t s, float x[8]) {
       const uint32_t ch = 4 * s + c4;
@@ -520,6 +527,7 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
         pb[t][0] = transpose8(take_term<BF16>(p[0], p[1]));
         pb[t][1] = transpose8(take_term<BF16>(p[2], p[3]));
       }
+      rows_v(cell);
 #pragma unroll
       for (int d = 0; d < KV; ++d) {
         const uint32_t v0[4] = {vr[0][d].x, vr[0][d].y, vr[0][d].z, vr[0][d].w};
@@ -544,8 +552,8 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
             for (int t = TP - 1; t >= 0; --t) mma16<BF16>(acc[d * 4 + j], av, pb[t][0], pb[t][1]);
           }
         }
+        load_v(d);
       }
-      load_v(cell);
     }
     // sums of the lane's two columns over the slots
 #pragma unroll

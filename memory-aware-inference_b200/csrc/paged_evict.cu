@@ -448,13 +448,14 @@ extern "C" int si_paged_evict_dev(si_ctx* ctx, const si_paged_kv* kv, const si_p
   const cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   const uint32_t rows = uint32_t(rows_of(*kv)), most = p.most;
   // A CTA for 8192 keys, as long as the clusters find room beside each other: a
-  // graphics processing cluster has 14 multiprocessors or more, so 8 of them
-  // hold 8, 24 or 56 clusters of 8, 4 or 2 CTAs for sure. (16 rows of 131,072: a
-  // second wave of clusters of 8 cost 35 us.)
-  uint32_t cluster = 1;
-  while (cluster < kMaxCluster && most > cluster * 8192 &&
-         (most > cluster * kCtaSlots || rows <= (cluster == 1 ? 56u : cluster == 2 ? 24u : 8u)))
-    cluster *= 2;
+  // graphics processing cluster has 14 multiprocessors or more, so 8 of them hold
+  // 8 (14 / c) clusters of c CTAs for sure. Multiprocessors come in pairs, and odd
+  // sizes were slower than the even ones on both sides (16 rows of 131,072 slots:
+  // clusters of 8, in two waves, 110 us; 7, 98; 6, 82; 5, 84; 4, 88).
+  uint32_t cluster = std::min(kMaxCluster, (most + 8191) / 8192);
+  if (cluster > 1) cluster += cluster % 2;
+  while (cluster > 1 && rows > 8 * (14 / cluster) && most <= (cluster > 2 ? cluster - 2 : 1) * kCtaSlots)
+    cluster = cluster > 2 ? cluster - 2 : 1;
   const uint32_t each = (most + cluster - 1) / cluster;
   // Moves of one row are at most the smaller of both sides of the budget. A few
   // (a page's worth leaves in steady state) the selecting CTA makes itself, which saves a
@@ -463,9 +464,11 @@ extern "C" int si_paged_evict_dev(si_ctx* ctx, const si_paged_kv* kv, const si_p
   // still read those.
   const uint64_t most_moves = std::min<uint64_t>(most > a->budget ? most - a->budget : 0, a->budget);
   p.at_once = cluster == 1 && most_moves <= 256 && p.len_in != p.len_out;
-  // 256, 512 or 1024 threads for about 16 keys a thread
-  const cudaError_t e = cluster > 1 ? (each > 8192 ? select<1024, true>(p, rows, cluster, each, s) : select<512, true>(p, rows, cluster, each, s))
-                        : each > 8192 ? select<1024, false>(p, rows, 1, each, s) : each > 2048 ? select<512, false>(p, rows, 1, each, s) : select<256, false>(p, rows, 1, each, s);
+  // 256, 512 or 1024 threads for up to 8 or 16 keys a thread; a cluster's CTAs have their multiprocessors to themselves
+  const cudaError_t e = cluster > 1   ? select<1024, true>(p, rows, cluster, each, s)
+                        : each > 8192 ? select<1024, false>(p, rows, 1, each, s)
+                        : each > 2048 ? select<512, false>(p, rows, 1, each, s)
+                                      : select<256, false>(p, rows, 1, each, s);
   if (e != cudaSuccess) return cuda_fail(ctx, e, "paged eviction launch");
   if (!p.at_once) {
     const uint64_t lanes = most_moves * kLanes;
