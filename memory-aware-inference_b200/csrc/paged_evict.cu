@@ -198,6 +198,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) evict_select
   // Keys; and the weights and positions below the new length go out as they
   // are (the second kernel writes over those of the holes).
   const int64_t next = a.next ? int64_t(a.next[b]) : int64_t(n);
+  // positions below `low` or from `high` on are protected (none reaches a `high` past 31 bits)
+  const int32_t low = int32_t(min(a.sink, 0x7fffffffu));
+  const int64_t from = next - int64_t(a.recent);
+  const int32_t high = int32_t(max(int64_t(INT32_MIN), min(from, int64_t(INT32_MAX))));
+  const bool any_high = from <= INT32_MAX;
   const bool w_copy = a.w_out != a.w_in, p_copy = a.p_out && a.p_out != a.p_in;
   const uint32_t stop = leave ? hi : min(hi, w_copy || p_copy ? m : 0);
   for (uint32_t i = tid; i < kBins; i += THREADS) s_bin[i] = 0;
@@ -215,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) evict_select
     for (uint32_t i = 0; i < 4; ++i) {
       const uint32_t t = t0 + i * THREADS;
       if (t >= stop) break;
-      const bool held = pos[i] < int64_t(a.sink) || pos[i] >= next - int64_t(a.recent);
+      const bool held = pos[i] < low || (any_high && pos[i] >= high);
       const uint32_t k = held ? kKeep : key_of(wt[i]);
       s_key[t - lo] = k;
       atomicAdd(&s_bin[k >> 21], 1u);
@@ -280,12 +285,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) evict_select
     if (same == want) break;  // the same in all threads of the cluster
   }
   // `want` of the keys equal to `found` leave, lowest slots first. A warp walks
-  // its own run of consecutive slots.
+  // its own run of consecutive slots, 32 a step.
   const uint32_t run = chunk / kWarps, w0 = min(hi, lo + w * run), w1 = min(hi, w0 + run);
-  auto walk = [&](auto&& body) {
-#pragma unroll 4
-    for (uint32_t t = w0; t < w1; t += 32) body(t + lane, t + lane < w1 ? s_key[t + lane - lo] : 0u, t + lane < w1);
-  };
   // v summed over the warps before this one, cluster-wide
   auto before_warp = [&](uint32_t v, uint32_t* s_total, uint32_t* cluster_total) {
     uint32_t total;
@@ -305,44 +306,68 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 2) evict_select
     *cluster_total = all;
     return before + __shfl_sync(0xffffffffu, mine, 0);
   };
-  // whether the lane's slot leaves; `seen`: equal keys before this row of slots
   const bool all_same = want == same;
   const uint32_t below = (1u << lane) - 1, limit = found | ~mask;  // all_same: everything up to `limit` leaves
-  uint32_t tie0 = 0, seen = 0, all;
-  auto leaves = [&](uint32_t k, bool in) {
-    if (all_same) return in && k <= limit;
-    const uint32_t eq = __ballot_sync(0xffffffffu, in && k == found);
-    const bool gone = in && (k < found || (k == found && seen + __popc(eq & below) < want));
-    seen += __popc(eq);
-    return gone;
-  };
+  uint32_t seen = 0, all;
   if (!all_same) {
     uint32_t ties = 0;
-    walk([&](uint32_t, uint32_t k, bool in) { ties += __popc(__ballot_sync(0xffffffffu, in && k == found)); });
-    tie0 = before_warp(ties, &s_ties, &all);
+#pragma unroll 4
+    for (uint32_t t = w0 + lane; t - lane < w1; t += 32)
+      ties += __popc(__ballot_sync(0xffffffffu, t < w1 && s_key[t - lo] == found));
+    seen = before_warp(ties, &s_ties, &all);  // equal keys before the warp's run
   }
+  // Bit l of word i of the run: slot 32 i + l leaves. The words go over the run's
+  // first keys, which the warp has read by then (a run has a word for 32 keys).
+  uint32_t* word = s_key + (w0 - lo);
+#pragma unroll 4
+  for (uint32_t t = w0 + lane; t - lane < w1; t += 32) {
+    const bool in = t < w1;
+    const uint32_t k = in ? s_key[t - lo] : kKeep;
+    uint32_t gone;
+    if (all_same) {
+      gone = __ballot_sync(0xffffffffu, in && k <= limit);
+    } else {
+      const uint32_t eq = __ballot_sync(0xffffffffu, in && k == found);
+      gone = __ballot_sync(0xffffffffu, in && (k < found || (k == found && seen + __popc(eq & below) < want)));
+      seen += __popc(eq);
+    }
+    if (lane == 0) word[(t - lane - w0) / 32] = gone;
+  }
+  __syncwarp();
+  // The words' holes below the new length, and kept slots behind it: a lane a word.
+  const uint32_t words = (w1 - w0 + 31) / 32;
+  auto bits_of = [&](uint32_t i, uint32_t& hole, uint32_t& stay) {
+    hole = stay = 0;
+    if (i >= words) return;
+    const uint32_t t = w0 + 32 * i, left = w1 - t;
+    const uint32_t in = left >= 32 ? 0xffffffffu : (1u << left) - 1;
+    const uint32_t kept_side = m <= t ? 0u : m - t >= 32 ? 0xffffffffu : (1u << (m - t)) - 1;
+    hole = word[i] & kept_side;
+    stay = ~word[i] & in & ~kept_side;
+  };
   uint32_t holes = 0, kept = 0;
-  seen = tie0;
-  walk([&](uint32_t t, uint32_t k, bool in) {
-    const bool gone = leaves(k, in);
-    holes += __popc(__ballot_sync(0xffffffffu, gone && t < m));
-    kept += __popc(__ballot_sync(0xffffffffu, in && !gone && t >= m));
-  });
+  for (uint32_t i = lane; i < words; i += 32) {
+    uint32_t hole, stay;
+    bits_of(i, hole, stay);
+    holes += __popc(hole);
+    kept += __popc(stay);
+  }
+  holes = __reduce_add_sync(0xffffffffu, holes);
+  kept = __reduce_add_sync(0xffffffffu, kept);
   uint32_t moved;
   uint32_t hole0 = before_warp(holes, &s_moves[0], &moved);
   uint32_t kept0 = before_warp(kept, &s_moves[1], &all);
-  seen = tie0;
-  uint32_t *from = a.moves + uint64_t(row) * 2 * a.room, *to = from + a.room;
-  if (__any_sync(0xffffffffu, holes | kept)) {
-    walk([&](uint32_t t, uint32_t k, bool in) {
-      const bool gone = leaves(k, in);
-      const bool hole = gone && t < m, mover = in && !gone && t >= m;
-      const uint32_t hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, mover);
-      if (hole) to[hole0 + __popc(hb & below)] = t;
-      if (mover) from[kept0 + __popc(mb & below)] = t;
-      hole0 += __popc(hb);
-      kept0 += __popc(mb);
-    });
+  uint32_t *from_list = a.moves + uint64_t(row) * 2 * a.room, *to_list = from_list + a.room;
+  if (holes | kept) {
+    for (uint32_t i = 0; i < words; ++i) {
+      uint32_t hole, stay;
+      bits_of(i, hole, stay);
+      const uint32_t t = w0 + 32 * i + lane;
+      if (hole >> lane & 1) to_list[hole0 + __popc(hole & below)] = t;
+      if (stay >> lane & 1) from_list[kept0 + __popc(stay & below)] = t;
+      hole0 += __popc(hole);
+      kept0 += __popc(stay);
+    }
   }
   if (rank == 0 && tid == 0) a.counts[row] = moved;
   if (!CLUSTER && a.at_once) {
