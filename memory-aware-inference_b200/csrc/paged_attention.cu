@@ -6,19 +6,22 @@
 // tokens are in the batch, and by latency below that.
 //
 // Split. The unit of work is 16 consecutive slots of one (sequence, kv head,
-// block of 8 query heads). All units of the batch, in that order, are shared
-// out evenly over the warps of one resident CTA a multiprocessor, whatever the
-// lengths: the counts come from lengths on the device, so a call needs no host
-// copy of them and a captured call follows later lengths. A warp's share covers
-// the end of one (sequence, head), some whole ones, and the beginning of
-// another; whole ones are written at once, the partial ones (at most two a
-// warp) meet in shared memory after the CTA's only barrier, those that cross
-// the CTA's borders (at most two a CTA) in the workspace, which a second
-// kernel joins. Every join sums in a fixed order.
+// block of 8 query heads), a pair. All units of the batch, in that order, are
+// shared out evenly over the workers of one resident CTA a multiprocessor,
+// whatever the lengths: the counts come from lengths on the device, so a call needs no
+// host copy of them and a captured call follows later lengths. A worker's share covers
+// the end of one pair, some whole ones, and the beginning of another; whole
+// ones are written at once, the partial ones (at most two a worker) meet in
+// shared memory at the end, those that cross the CTA's borders (at most two a
+// CTA) in the workspace, which a second kernel joins. Every join sums in a fixed order.
+// A worker is a warp; for head_dim above 192 two warps, each with half of the
+// dims, that exchange their halves of the scores once a unit (one call of 517
+// slots of 256 dims 13.6 us where one warp a unit takes 14.8, 65,536 slots with bf16
+// queries 53 and 56, 131,071 with f32 ones 110 and 107).
 //
 // A unit. Keys and values go from global memory straight into the registers
 // in which the tensor cores (mma.m16n8k16) want them; there is no shared-memory
-// stage and no barrier in the loop:
+// stage:
 //   S^T = K Q^T: the order of dims in the contraction is free as long as both
 //     operands share it, so a lane's 16-byte load of 8 dims of a key is the A
 //     operand of two steps. Lane (n, c) = (lane / 4, lane % 4) loads dims
@@ -31,7 +34,9 @@
 //   P leaves the first product transposed; movmatrix turns it into the second
 //     one's B operand.
 // The keys of the next unit are requested when this unit's scores are done,
-// its values after this unit's product, so loads are in flight throughout.
+// its values step by step as this unit's are used, so loads are in flight
+// throughout. What bounds it: HBM for 16-bit queries (64 ragged sequences, 0.69 GB
+// in 112 us, 6.2 TB/s), the latency of a unit for f32 ones (0.54 GB in 110 us).
 //
 // Precision: queries are split into TQ 16-bit terms and probabilities into TP,
 // each multiplied separately into the same f32 accumulators. 16-bit queries of
@@ -64,8 +69,11 @@ constexpr float shift_of(bool bf16) { return bf16 ? 0.f : 11.f; }
 
 template <int HD>
 struct Shape {
-  static constexpr int kWarps = HD <= 128 ? 12 : 8;  // registers: 168 or 255 a thread
-  static constexpr int kK = HD / 32, kV = HD / 64;   // 16-byte loads a slot and lane
+  static constexpr int kSplit = HD > 192 ? 2 : 1;      // warps of a worker, a share of the dims each
+  static constexpr int kDims = HD / kSplit;
+  static constexpr int kWarps = kDims <= 128 ? 12 : 8;   // registers: 168 or 255 a thread
+  static constexpr int kWorkers = kWarps / kSplit;
+  static constexpr int kK = kDims / 32, kV = kDims / 64; // 16-byte loads a slot and lane
 };
 
 // Join records and partials in the workspace (one CTA: two partial slots).
@@ -260,21 +268,23 @@ __device__ __forceinline__ void finish(const AttArgs& a, const Place& at, uint32
 
 template <int HD, bool BF16, int TQ, int TP>
 __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_kernel(const __grid_constant__ AttArgs a) {
-  constexpr int NW = Shape<HD>::kWarps, KK = Shape<HD>::kK, KV = Shape<HD>::kV;
+  using Sh = Shape<HD>;
+  constexpr int NW = Sh::kWarps, WK = Sh::kWorkers, KK = Sh::kK, KV = Sh::kV;
   constexpr float kShift = shift_of(BF16);
   constexpr uint32_t kPart = kCols * (HD + 2);                   // floats of a partial: values, then max and sum
   constexpr uint32_t kQ = uint32_t(TQ * KK) * 32 * 4;            // floats of a warp's query terms
-  constexpr uint32_t kRegion = (kQ > kPart ? kQ : kPart) + kPart;
+  constexpr uint32_t kRegion = (kQ * Sh::kSplit > kPart ? kQ * Sh::kSplit : kPart) + kPart;
   extern __shared__ __align__(16) float smem[];
-  // per warp: [query terms, later the partial of the last pair][partial of the first pair]
+  // per worker: [query terms, later the partial of the last pair][partial of the first pair]
   __shared__ uint32_t s_warp[NW];
-  __shared__ Place s_part[2 * NW];  // pairs of the warps' partials; tiles 0: no partial
+  __shared__ Place s_part[2 * WK];  // pairs of the workers' partials; tiles 0: no partial
+  __shared__ float4 s_half[Sh::kSplit > 1 ? WK : 1][2][Sh::kSplit][32];  // scores over a share of the dims
   __shared__ uint8_t s_list[32], s_lead[32];
   __shared__ uint32_t s_leads;
-  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + NW * kRegion);
+  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + WK * kRegion);
   const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5, n8 = lane >> 2, c4 = lane & 3;
   const uint32_t heads = a.kv.kv_heads * a.blocks;
-  if (threadIdx.x < 2 * NW) s_part[threadIdx.x].tiles = 0;
+  if (threadIdx.x < 2 * WK) s_part[threadIdx.x].tiles = 0;
   pdl_launch_dependents();
   pdl_wait();
   step_prefix(a, prefix, s_warp);
@@ -290,20 +300,28 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
     if (a.lse)
       for (uint32_t h = threadIdx.x; h < a.qh; h += NW * 32) a.lse[uint64_t(b) * a.qh + h] = -INFINITY;
   }
-  // little work: fewer CTAs, so that most warps still have a unit
-  const uint32_t ctas = min(gridDim.x, (steps + NW - 1) / NW), cta = blockIdx.x;
+  // little work: fewer CTAs, so that most workers still have a unit
+  const uint32_t ctas = min(gridDim.x, (steps + WK - 1) / WK), cta = blockIdx.x;
   if (cta >= ctas) {
     if (threadIdx.x == 0) a.join[cta].last = -1;
     return;
   }
-  const Shares cta_share(steps, ctas), warp_share(steps, ctas * NW);
+  const Shares cta_share(steps, ctas), worker_share(steps, ctas * WK);
   const uint32_t cu0 = cta_share.begin(cta), cu1 = cta_share.begin(cta + 1);
-  const uint32_t u0 = warp_share.begin(cta * NW + w), u1 = warp_share.begin(cta * NW + w + 1);
-  float* region = smem + w * kRegion;
-  uint4* s_q = reinterpret_cast<uint4*>(region) + lane;  // [step][term][lane]: a lane reads what it wrote
-  const uint32_t chunks = a.kv.hd / 8;
+  const uint32_t worker = w / Sh::kSplit, half = w % Sh::kSplit, dim0 = half * Sh::kDims;
+  const uint32_t u0 = worker_share.begin(cta * WK + worker), u1 = worker_share.begin(cta * WK + worker + 1);
+  float* region = smem + worker * kRegion;
+  uint4* s_q = reinterpret_cast<uint4*>(region + half * kQ) + lane;  // [step][term][lane]: a lane reads what it wrote
+  const uint32_t chunks = a.kv.hd / 8, mine = min(uint32_t(Sh::kDims / 8), chunks - dim0 / 8);
   // steps in which the lane has dims below head_dim
-  const uint32_t k_steps = (chunks + 3 - c4) / 4, v_steps = (chunks + 7 - n8) / 8;
+  const uint32_t k_steps = (mine + 3 - c4) / 4, v_steps = (mine + 7 - n8) / 8;
+  auto worker_sync = [&] {
+    if constexpr (Sh::kSplit == 1)
+      __syncwarp();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + worker), "n"(Sh::kSplit * 32) : "memory");
+  };
+  uint32_t flip = 0;  // which half of s_half the next unit uses
 
   Place at;
   if (u0 < u1) at = place_of(u0, prefix, a.kv.sequences, heads);
@@ -327,13 +345,13 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
     // Queries as they are, each lane's own into its places of shared memory;
     // rolled loops here and at the pair's end: code that runs once a pair costs
     // its instruction fetches.
-    const uint64_t q0 = at.b * a.q_ss + uint64_t(qhead0 + n8) * a.q_hs;
+    const uint64_t q0 = at.b * a.q_ss + uint64_t(qhead0 + n8) * a.q_hs + dim0;
     if (a.q_wide) {
       const uint8_t* from = static_cast<const uint8_t*>(a.q) + q0 * elem_bytes(a.elem);
 #pragma unroll 1
       for (uint32_t s = 0; s < KK; ++s) {
         const uint32_t ch = 4 * s + c4;
-        const bool on = n8 < cols && ch < chunks;
+        const bool on = n8 < cols && ch < mine;
         const uint8_t* x = on ? from + ch * 8 * elem_bytes(a.elem) : static_cast<const uint8_t*>(a.q);
         cp_async16(s_q + s * TQ * 32, x, on);
         if (TQ > 1 && a.elem == SI_ELEM_F32) cp_async16(s_q + (s * TQ + 1) * 32, on ? x + 16 : x, on);
@@ -350,7 +368,7 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
       const uint64_t c0 = shfl64(cell, n8), c1 = shfl64(cell, n8 + 8);
       lo = c0 != kNoCell;
       hi = c1 != kNoCell;
-      const uint16_t *p0 = a.kv.k + c0 + c4 * 8, *p1 = a.kv.k + c1 + c4 * 8;
+      const uint16_t *p0 = a.kv.k + c0 + dim0 + c4 * 8, *p1 = a.kv.k + c1 + dim0 + c4 * 8;
       const uint32_t n0 = lo ? k_steps : 0, n1 = hi ? k_steps : 0;
 #pragma unroll
       for (uint32_t s = 0; s < KK; ++s) {
@@ -367,7 +385,7 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t c = shfl64(cell, 2 * c4 + (i & 1) + (i >> 1) * 8);
-        vp[i] = a.kv.v + c + n8 * 8;
+        vp[i] = a.kv.v + c + dim0 + n8 * 8;
         vn[i] = c != kNoCell ? v_steps : 0;
       }
     };
@@ -400,7 +418,7 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = elem_to_f(uint16_t(h[j / 2] >> (j % 2 * 16)), a.elem);
         }
-      } else if (n8 < cols && ch < chunks) {
+      } else if (n8 < cols && ch < mine) {
         load8(a.q, q0 + ch * 8, a.elem, false, x);
       } else {
 #pragma unroll
@@ -476,16 +494,23 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
         for (int t = TQ - 1; t > 0; --t) low += chain[2 * t - 1][i] + chain[2 * t][i];
         s[i] += chain[0][i] + low;
       }
+      // base-2 scores; over half of the dims, the other half's are added
+      s[0] *= sc0, s[1] *= sc1, s[2] *= sc0, s[3] *= sc1;
+      if constexpr (Sh::kSplit > 1) s_half[worker][flip][half][lane] = make_float4(s[0], s[1], s[2], s[3]);
       const bool lo_now = lo, hi_now = hi;
       cell = cell_of(tile + 1, page_next);
       page_next = page_after;
       load_k(cell, lo, hi);
-      // base-2 scores; slots that do not exist leave nothing
-      s[0] = lo_now ? s[0] * sc0 : -INFINITY;
-      s[1] = lo_now ? s[1] * sc1 : -INFINITY;
-      s[2] = hi_now ? s[2] * sc0 : -INFINITY;
-      s[3] = hi_now ? s[3] * sc1 : -INFINITY;
-      if (a.scores) {
+      if constexpr (Sh::kSplit > 1) {
+        worker_sync();  // the only one a unit: the other half of s_half is used next
+        const float4 x = s_half[worker][flip][0][lane], y = s_half[worker][flip][1][lane];
+        s[0] = x.x + y.x, s[1] = x.y + y.y, s[2] = x.z + y.z, s[3] = x.w + y.w;
+        flip ^= 1;
+      }
+      // slots that do not exist leave nothing
+      if (!lo_now) s[0] = s[1] = -INFINITY;
+      if (!hi_now) s[2] = s[3] = -INFINITY;
+      if (a.scores && half == 0) {
         float* to = a.scores + (uint64_t(at.b * a.kv.kv_heads + kvh) * a.kv.max_tokens + tile * kUnit) * a.gpad + col0 + 2 * c4;
         if (2 * c4 < cols) {  // gpad is even: the pair's second place exists
           if (tile * kUnit + n8 < len) *reinterpret_cast<float2*>(to + uint64_t(n8) * a.gpad) = make_float2(s[0], s[1]);
@@ -566,32 +591,33 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
     const bool whole = t_begin == 0 && t_end == at.tiles;
     const uint32_t slot = u == u0 && !whole ? 0 : 1;
     float* part = slot ? region : region + (kRegion - kPart);
-    __syncwarp();
+    worker_sync();  // all have read their queries
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const uint32_t col = 2 * c4 + c;
 #pragma unroll
       for (int d = 0; d < KV; ++d) {
-        float* to = part + col * HD + (8 * d + n8) * 8;
+        float* to = part + col * HD + dim0 + (8 * d + n8) * 8;
         *reinterpret_cast<float4*>(to) =
             make_float4(acc[d * 4][c], acc[d * 4][2 + c], acc[d * 4 + 1][c], acc[d * 4 + 1][2 + c]);
         *reinterpret_cast<float4*>(to + 4) =
             make_float4(acc[d * 4 + 2][c], acc[d * 4 + 2][2 + c], acc[d * 4 + 3][c], acc[d * 4 + 3][2 + c]);
       }
-      if (n8 == 0) *reinterpret_cast<float2*>(part + kCols * HD + 2 * col) = make_float2(c ? m1 : m0, c ? l1 : l0);
+      if (n8 == 0 && half == 0)
+        *reinterpret_cast<float2*>(part + kCols * HD + 2 * col) = make_float2(c ? m1 : m0, c ? l1 : l0);
     }
     if (!whole) {
-      if (lane == 0) s_part[2 * w + slot] = at;
+      if (half == 0 && lane == 0) s_part[2 * worker + slot] = at;
       continue;
     }
-    __syncwarp();
+    worker_sync();
 #pragma unroll 1
-    for (uint32_t i = lane; i < cols * chunks; i += 32) {
+    for (uint32_t i = half * 32 + lane; i < cols * chunks; i += Sh::kSplit * 32) {
       const uint32_t col = i / chunks, ch = i - col * chunks;
       const float2 ml = *reinterpret_cast<const float2*>(part + kCols * HD + 2 * col);
       finish<HD>(a, at, qhead0 + col, ch, ml.x - kShift, ml.y, part + col * HD + ch * 8);
     }
-    __syncwarp();
+    worker_sync();
   }
   if (threadIdx.x == 0) {
     Join j = {-1, 0, 0, 0};
@@ -611,11 +637,11 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
     a.join[cta] = j;
   }
   __syncthreads();
-  // Join the warps' partials in the order of their units. Warp 0 lists them:
+  // Join the workers' partials in the order of their units. Warp 0 lists them:
   // s_list[k] is the k-th partial, s_lead[i] the first one of the i-th pair.
   if (w == 0) {
-    const Place p = s_part[lane < 2 * NW ? lane : 0];
-    const bool on = lane < 2 * NW && p.tiles != 0;
+    const Place p = s_part[lane < 2 * WK ? lane : 0];
+    const bool on = lane < 2 * WK && p.tiles != 0;
     const uint32_t all = __ballot_sync(0xffffffffu, on), below = all & ((1u << lane) - 1);
     const uint32_t before = __shfl_sync(0xffffffffu, p.begin, below ? 31 - __clz(below) : 0);
     const uint32_t leads = __ballot_sync(0xffffffffu, on && (!below || before != p.begin));
@@ -767,7 +793,7 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(const __grid_constan
 }
 
 uint32_t padded_dim(uint32_t hd) { return (hd + 63) / 64 * 64; }
-uint32_t warps_of(uint32_t hd) { return padded_dim(hd) <= 128 ? 12 : 8; }
+uint32_t workers_of(uint32_t hd) { return padded_dim(hd) <= 128 ? 12 : padded_dim(hd) <= 192 ? 8 : 6; }
 
 // Workspace: join records, partials, then lse and scores of the weights pass.
 // The grid is one CTA a multiprocessor, so kMaxCtas bounds both.
@@ -831,9 +857,10 @@ int check_attention(const si_paged_kv* kv, const si_paged_attention* a, std::str
 
 template <int HD, bool BF16, int TQ, int TP>
 cudaError_t launch(const AttArgs& p, uint32_t grid, cudaStream_t s) {
-  constexpr uint32_t kPart = kCols * (HD + 2), kQ = uint32_t(TQ * (HD / 32)) * 32 * 4;
+  using Sh = Shape<HD>;
+  constexpr uint32_t kPart = kCols * (HD + 2), kQ = uint32_t(TQ * Sh::kK) * 32 * 4 * Sh::kSplit;
   constexpr uint32_t kRegion = (kQ > kPart ? kQ : kPart) + kPart;
-  const uint32_t smem = Shape<HD>::kWarps * kRegion * 4 + (p.kv.sequences + 1) * 4;
+  const uint32_t smem = Sh::kWorkers * kRegion * 4 + (p.kv.sequences + 1) * 4;
   static std::atomic<uint32_t> cache[kMaxDevices];
   auto kernel = paged_attention_kernel<HD, BF16, TQ, TP>;
   if (cudaError_t e = raise_smem_limit(kernel, smem, cache)) return e;
@@ -898,7 +925,7 @@ extern "C" int si_paged_attention_dev(si_ctx* ctx, const si_paged_kv* kv, const 
   }
   const cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   const uint64_t most = most_steps(*kv, p.qh);
-  const uint32_t nw = warps_of(kv->head_dim);
+  const uint32_t nw = workers_of(kv->head_dim);
   const uint32_t grid = uint32_t(std::min<uint64_t>(std::min<uint32_t>(ctx->sm_count, kMaxCtas), (most + nw - 1) / nw));
   const bool bf16 = kv->elem == SI_ELEM_BF16;
   cudaError_t e;

@@ -801,3 +801,168 @@ def test_drafts_over_the_paged_cache(ctx):
     assert (accepted.item(), following.item()) == (want[0], verified(p[0].cpu().numpy(), None, tokens[0].tolist(), u[0].tolist(),
                                                                      last.item(), k_drafts)[1])
     ctx.synchronize()
+
+
+# ---- calls that the documentation allows and that come up seldom ------------------------------
+@pytest.mark.parametrize("hd", [136, 184, 200, 248])
+@pytest.mark.parametrize("io, cache_type", [(F32, BF16), (BF16, BF16), (F32, F16)])
+def test_attention_odd_heads(ctx, hd, io, cache_type):
+    """Heads that leave part of the last steps empty, long and short rows, whole pairs and split ones."""
+    cache = Cache([700, 0, 1, 33, 16, 5000], 2, 16, hd, cache_type, seed=hd, order="tokens_first")
+    q = torch.randn(6, 14, hd, device="cuda").to(io)
+    close(attend(ctx, cache, q), reference(cache, q)[0], io)
+
+
+def test_attention_many_short_sequences(ctx):
+    """The most sequences that a call takes, most of them empty or of one token."""
+    lengths = [(0, 1, 0, 2, 17)[i % 5] for i in range(4096)]
+    cache = Cache(lengths, 1, 16, 64, BF16, seed=1)
+    q = torch.randn(4096, 2, 64, device="cuda")
+    out = attend(ctx, cache, q)
+    want, _, _ = reference(cache, q)
+    close(out, want, F32)
+    assert (out[::5] == 0).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_keeps_rows_apart(ctx, hd, bad):
+    """A sequence whose cache or query holds NaN or infinity leaves the others alone, in the same warp or not."""
+    lengths = [20, 7, 300, 5, 1, 0, 40, 33]
+    for io, cache_type in ((F32, BF16), (F16, F16)):
+        cache = Cache(lengths, 2, 16, hd, cache_type, seed=hd)
+        q = torch.randn(8, 4, hd, device="cuda").to(io)
+        want, _, _ = reference(cache, q)
+        for b, pool in ((1, cache.k), (3, cache.v), (6, cache.k)):
+            pg, at = cache.cells(b, lengths[b])
+            pool[pg, :, at] = bad
+        q[4] = bad
+        out = attend(ctx, cache, q)
+        good = [0, 2, 5, 7]
+        close(out[good], want[good], io)
+        assert not torch.isfinite(out[[3, 4]]).any()
+
+
+def test_operators_on_streams_of_their_own(ctx):
+    """All four operators on four streams at once, twenty times, with workspaces of their own."""
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    att = Cache([900, 33, 0], 2, 16, 128, BF16, seed=1)
+    q = torch.randn(3, 8, 128, device="cuda")
+    out = torch.empty_like(q)
+    attention = mai.paged_attention(att.desc, q, out, att.len_dev, work_for(att, 8))
+    app = Cache([40] * 4, 2, 8, 64, BF16, seed=2)
+    new, slot = torch.randn(4, 2, 64, device="cuda").to(BF16), torch.tensor([3, 39, 0, 17], dtype=torch.int32, device="cuda")
+    append = mai.paged_append(app.desc, None, new, new, None, slot)
+    ev = Cache([600, 20], 2, 16, 64, F16, seed=3)
+    w = torch.rand(2, 2, 640, device="cuda")
+    w_out, n_out = torch.zeros_like(w), torch.zeros_like(ev.len_dev)
+    evict = mai.paged_evict(ev.desc, ev.len_dev, n_out, w, w_out, 500,
+                            torch.empty(mai.paged_evict_workspace_bytes(ev.desc), dtype=torch.uint8, device="cuda"), recent=50)
+    p = torch.rand(5, 4, 3001, device="cuda")
+    tokens, u, last = torch.zeros(5, 3, dtype=torch.int32, device="cuda"), torch.rand(5, 3, device="cuda"), torch.rand(5, device="cuda")
+    accepted, following = (torch.zeros(5, dtype=torch.int32, device="cuda") for _ in range(2))
+    verify = mai.verify_drafts(p, tokens, u, last, accepted, following, torch.empty(16, dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        ctx.paged_attention_dev(att.desc, attention, streams[0].cuda_stream)
+        ctx.paged_append_dev(app.desc, append, streams[1].cuda_stream)
+        ctx.paged_evict_dev(ev.desc, evict, streams[2].cuda_stream)
+        ctx.verify_drafts_dev(verify, streams[3].cuda_stream)
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    close(out, reference(att, q)[0], F32)
+    for b, t in enumerate(slot.tolist()):
+        assert torch.equal(app.k[app.pages[b, t // 8].item(), :, t % 8], new[b])
+    assert n_out.tolist() == [500, 20]
+    for h in range(2):
+        holes, movers = evicted(w[0, h].tolist(), list(range(640)), 600, 500, 0, 50, 600)
+        got = w[0, h, :500].clone()
+        got[holes] = w[0, h, movers]
+        assert torch.equal(w_out[0, h, :500], got)
+    for b in range(5):
+        assert (accepted[b].item(), following[b].item()) == verified(p[b].cpu().numpy(), None, tokens[b].tolist(), u[b].tolist(),
+                                                                     last[b].item(), 3)
+
+
+@pytest.mark.parametrize("leave", [30, 700])
+def test_evict_captured_in_place(ctx, leave):
+    """A captured call over its own lengths: the first replay cuts, the next ones find nothing to do."""
+    n, budget = 2000, 2000 - leave
+    cache = Cache([n, 100], 2, 16, 64, BF16, seed=leave)
+    w = torch.rand(2, 2, n, device="cuda")
+    pos = torch.arange(n, dtype=torch.int32, device="cuda").expand(2, 2, n).contiguous()
+    length, before = cache.len_dev, w.clone()
+    work = torch.empty(mai.paged_evict_workspace_bytes(cache.desc), dtype=torch.uint8, device="cuda")
+    args = mai.paged_evict(cache.desc, length, length, w, w, budget, work, sink=4, recent=16, positions_in=pos, positions_out=pos)
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        ctx.paged_evict_dev(cache.desc, args, s.cuda_stream)
+    k0 = cache.k.clone()
+    for turn in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert length.tolist() == [budget, 100]
+        for h in range(2):
+            holes, movers = evicted(before[0, h].tolist(), list(range(n)), n, budget, 4, 16, n)
+            want = list(range(budget))
+            for a, b in zip(holes, movers):
+                want[a] = b
+            assert pos[0, h, :budget].tolist() == want
+            assert torch.equal(w[0, h, :budget], before[0, h, want])
+            pg, at = cache.cells(0, n)
+            assert torch.equal(cache.k[pg[:budget], h, at[:budget]], k0[pg[want], h, at[want]])
+        assert torch.equal(w[1], before[1])
+
+
+def test_append_captured_follows_positions(ctx):
+    cache = Cache([64, 64], 2, 8, 64, BF16, seed=5)
+    table, _ = mai.rope_table(1e5, 64)
+    rope = torch.from_numpy(table.view(np.int64)).cuda()
+    q, k = torch.randn(2, 4, 64, device="cuda"), torch.randn(2, 2, 64, device="cuda")
+    out, slot = torch.empty_like(q), torch.zeros(2, dtype=torch.int32, device="cuda")
+    args = mai.paged_append(cache.desc, q, k, k, out, slot, rope=rope, rotary_dim=64, layout="half")
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        ctx.paged_append_dev(cache.desc, args, s.cuda_stream)
+    for slots in ([0, 63], [5, -1], [17, 40]):
+        slot.copy_(torch.tensor(slots))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        angle = torch.tensor([[max(t, 0) * int(f) / 2.0 ** 64 * 2 * math.pi for f in table] for t in slots], dtype=torch.float64).cuda()
+        want, keys = rotated(q, angle, "half", 1.0), rotated(k, angle, "half", 1.0)
+        for b, t in enumerate(slots):
+            if t < 0:
+                assert (out[b] == 7).all()
+                continue
+            close(out[b], want[b], F32)
+            close(cache.k[cache.pages[b, t // 8].item(), :, t % 8], keys[b], BF16)
+
+
+@pytest.mark.parametrize("vocab", [300, 9000, 100003])
+def test_verify_draws_from_the_target_when_nothing_is_left(ctx, vocab):
+    """The drafter's row is the target's: a token of no weight is rejected, and the row itself is drawn from."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    p = torch.softmax(torch.randn(7, 3, vocab, device="cuda", generator=gen), -1)
+    p[:, :, 11] = 0
+    q = p[:, :2].clone()
+    tokens = torch.full((7, 2), 11, dtype=torch.int32, device="cuda")
+    u, last = torch.rand(7, 2, device="cuda", generator=gen), torch.linspace(0, 0.999, 7, device="cuda")
+    accepted, following = run_verify(ctx, p, q, tokens, u, last)
+    for b in range(7):
+        assert (accepted[b].item(), following[b].item()) == verified(p[b].cpu().numpy(), q[b].cpu().numpy(), tokens[b].tolist(),
+                                                                     u[b].tolist(), last[b].item(), 2)
+
+
+def test_tensors_of_another_device_are_refused(ctx):
+    cache = Cache([4], 1, 4, 64)
+    host = mai.paged_kv(cache.k.cpu(), cache.v.cpu(), cache.pages)
+    q, n = torch.zeros(1, 1, 64), torch.zeros(1, dtype=torch.int32)
+    args = mai.paged_attention(host, q, q, n, torch.empty(1 << 22, dtype=torch.uint8))
+    with pytest.raises(mai.SiError):
+        ctx.paged_attention_dev(host, args, LEGACY)
+    with pytest.raises(mai.SiError):
+        mai.paged_attention(cache.desc, q, q, n, torch.empty(1 << 22, dtype=torch.uint8))

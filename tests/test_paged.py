@@ -280,6 +280,10 @@ def test_more_refusals():
     refused(L.si_paged_evict_dev, kv, a, status=UNSUPPORTED)
     with pytest.raises(mai.SiError):
         mai.paged_evict_workspace_bytes(kv)
+    kv, a = attention_call()
+    kv.sequences, kv.kv_heads, kv.page_tokens, kv.max_pages, kv.pages_stride = 256, 2, 1 << 20, 1 << 10, 1 << 10
+    a.query_heads = 1 << 15  # 2^24 units of 256 sequences, 2 kv heads and 2048 blocks of query heads
+    refused(L.si_paged_attention_dev, kv, a, status=UNSUPPORTED)
     kv, a = append_call()
     a.q += 2
     refused(L.si_paged_append_dev, kv, a)
