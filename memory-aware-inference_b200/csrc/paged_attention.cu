@@ -36,7 +36,7 @@
 // The keys of the next unit are requested when this unit's scores are done,
 // its values step by step as this unit's are used, so loads are in flight
 // throughout. What bounds it: HBM for 16-bit queries (64 ragged sequences, 0.69 GB
-// in 112 us, 6.2 TB/s), the latency of a unit for f32 ones (0.54 GB in 110 us).
+// in 115 us, 6.0 TB/s), the latency of a unit for f32 ones (0.54 GB in 114 us).
 //
 // Precision: queries are split into TQ 16-bit terms and probabilities into TP,
 // each multiplied separately into the same f32 accumulators. 16-bit queries of
