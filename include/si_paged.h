@@ -139,7 +139,7 @@ int si_paged_append_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_appen
  * weights_out, or NULL for zeros. */
 typedef struct si_paged_attention {
   const void* q;            /* [sequences][query_heads][head_dim] */
-  void* out;
+  void* out;                /* not q: several blocks read a query */
   uint64_t q_seq_stride, q_head_stride, out_seq_stride, out_head_stride;
   const int32_t* lengths;   /* [sequences], each at most max_pages * page_tokens */
   float scale;              /* 0: 1 / sqrt(head_dim) */
@@ -176,7 +176,7 @@ typedef struct si_paged_evict {
   float* weights_out;
   const int32_t* positions_in;  /* as weights_in; NULL: slot t holds position t */
   int32_t* positions_out;       /* NULL: not wanted */
-  const int32_t* next_position; /* [sequences]; NULL: lengths_in */
+  const int32_t* next_position; /* [sequences]; NULL: lengths_in. Not lengths_out, unless all three are one */
   uint64_t weights_stride;      /* of all four, entries; at least the longest length */
   uint32_t budget;              /* at least 1 */
   uint32_t sink, recent;        /* sink + recent <= budget */
@@ -208,7 +208,7 @@ typedef struct si_verify_drafts {
   const int32_t* counts;    /* [sequences] drafts of each sequence, at most `drafts`; NULL: all */
   const float* uniform;     /* [sequences][drafts] in [0, 1) */
   const float* last_uniform;/* [sequences] in [0, 1) */
-  int32_t* accepted;        /* [sequences] */
+  int32_t* accepted;        /* [sequences]; may be counts */
   int32_t* next;            /* [sequences] */
   uint32_t sequences;       /* at most 65535 */
   uint32_t drafts;          /* 0..32 */

@@ -811,24 +811,28 @@ class CudaContext:
                                               stream))
 
     # -- paged cache (include/si_paged.h; descriptions from paged.py) ---------
-    def _here(self, described):
-        """Refuses a description whose tensors are not on this context's GPU."""
-        if getattr(described, "_device", self.device) != self.device:
-            raise SiError(SI_E_INVALID, f"tensors are on {described._tensors[0].device}, the context on cuda:{self.device}")
+    def _here(self, *described):
+        """Refuses descriptions whose tensors are not on this context's GPU, and a
+        call whose tensors do not have its cache's sizes."""
+        for d in described:
+            if getattr(d, "_device", self.device) != self.device:
+                raise SiError(SI_E_INVALID, f"tensors are on {d._tensors[0].device}, the context on cuda:{self.device}")
+        if len(described) == 2:
+            described[1].check_cache(described[0])
 
     def paged_append_dev(self, kv: SiPagedKv, append: SiPagedAppend, stream=None):
         """si_paged_append_dev: rotary positions of new queries and keys, keys and values into pages."""
-        self._here(kv)
+        self._here(kv, append)
         self._ck(lib().si_paged_append_dev(self.h, C.byref(kv), C.byref(append), stream))
 
     def paged_attention_dev(self, kv: SiPagedKv, attention: SiPagedAttention, stream=None):
         """si_paged_attention_dev: attention of one new token a sequence over pages."""
-        self._here(kv)
+        self._here(kv, attention)
         self._ck(lib().si_paged_attention_dev(self.h, C.byref(kv), C.byref(attention), stream))
 
     def paged_evict_dev(self, kv: SiPagedKv, evict: SiPagedEvict, stream=None):
         """si_paged_evict_dev: every longer sequence cut to the budget by accumulated weight."""
-        self._here(kv)
+        self._here(kv, evict)
         self._ck(lib().si_paged_evict_dev(self.h, C.byref(kv), C.byref(evict), stream))
 
     def verify_drafts_dev(self, drafts: SiVerifyDrafts, stream=None):

@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <initializer_list>
 #include <string>
 
 #include "../../include/si_paged.h"
@@ -161,6 +162,12 @@ inline bool wide_ok(const void* p, uint32_t elem, uint64_t s0, uint64_t s1) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s0 % unit == 0 && s1 % unit == 0;
 }
 inline bool elem_aligned(const void* p, uint32_t elem) { return reinterpret_cast<uintptr_t>(p) % elem_bytes(elem) == 0; }
+// Arrays of 32-bit numbers (null ones count as aligned).
+inline bool words_aligned(std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if (reinterpret_cast<uintptr_t>(p) % 4) return false;
+  return true;
+}
 inline bool elem_known(uint32_t elem) { return elem <= SI_ELEM_F16; }
 
 // Makes the context's device current for the launches of one call.

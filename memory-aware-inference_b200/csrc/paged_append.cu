@@ -227,6 +227,8 @@ int check_append(const si_paged_kv* kv, const si_paged_append* a, std::string* m
     return bad(SI_E_INVALID, "paged append has more tokens than sequences and no sequence numbers");
   for (const void* p : {a->q, static_cast<const void*>(a->q_out), a->k, a->v})
     if (!elem_aligned(p, a->elem)) return bad(SI_E_INVALID, "paged append buffers are not aligned to their elements");
+  if (!words_aligned({a->sequence, a->slot, a->position}))
+    return bad(SI_E_INVALID, "paged append arrays of 32-bit numbers are not aligned");
   const uint64_t strides[] = {a->q_token_stride,     a->q_head_stride, a->q_out_token_stride, a->q_out_head_stride,
                               a->k_token_stride,     a->k_head_stride, a->v_token_stride,     a->v_head_stride};
   for (uint64_t s : strides)

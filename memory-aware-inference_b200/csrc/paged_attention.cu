@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(Shape<HD>::kWarps * 32, 1) paged_attention_ker
       for (uint32_t h = threadIdx.x; h < a.qh; h += NW * 32) a.lse[uint64_t(b) * a.qh + h] = -INFINITY;
   }
   // little work: fewer CTAs, so that most workers still have a unit
-  const uint32_t ctas = min(gridDim.x, (steps + WK - 1) / WK), cta = blockIdx.x;
+  const uint32_t ctas = min(gridDim.x, steps / WK + (steps % WK != 0)), cta = blockIdx.x;
   if (cta >= ctas) {
     if (threadIdx.x == 0) a.join[cta].last = -1;
     return;
@@ -840,7 +840,9 @@ int check_attention(const si_paged_kv* kv, const si_paged_attention* a, std::str
   if (int rc = check_heads(kv, a->query_heads, msg)) return rc;
   if (!elem_known(a->elem)) return bad(SI_E_UNSUPPORTED, "paged attention elements must be f32, bf16 or f16");
   if (!a->q || !a->out || !a->lengths) return bad(SI_E_INVALID, "paged attention buffers are null");
-  if (!elem_aligned(a->q, a->elem) || !elem_aligned(a->out, a->elem))
+  if (a->q == a->out) return bad(SI_E_INVALID, "paged attention cannot write its output over the queries");
+  if (!elem_aligned(a->q, a->elem) || !elem_aligned(a->out, a->elem) ||
+      !words_aligned({a->lengths, a->lse, a->weights_in, a->weights_out}))
     return bad(SI_E_INVALID, "paged attention buffers are not aligned to their elements");
   if (!(a->scale >= 0.f) || a->scale > 3e38f) return bad(SI_E_INVALID, "paged attention scale must be finite and not negative");
   if (a->weights_in && !a->weights_out) return bad(SI_E_INVALID, "paged attention has weights in and none out");

@@ -428,8 +428,13 @@ int check_evict(const si_paged_kv* kv, const si_paged_evict* a, std::string* msg
   if (int rc = check_size(kv, msg)) return rc;
   if (!a->lengths_in || !a->lengths_out || !a->weights_in || !a->weights_out)
     return bad(SI_E_INVALID, "paged eviction buffers are null");
+  if (!words_aligned({a->lengths_in, a->lengths_out, a->weights_in, a->weights_out, a->positions_in, a->positions_out,
+                      a->next_position}))
+    return bad(SI_E_INVALID, "paged eviction buffers are not aligned to their elements");
   if (a->positions_in && !a->positions_out)
     return bad(SI_E_INVALID, "paged eviction has positions in and none out");
+  if (a->next_position && a->next_position == a->lengths_out && a->lengths_in != a->lengths_out)
+    return bad(SI_E_INVALID, "paged eviction would write the new lengths over the next positions");
   if (a->budget == 0 || uint64_t(a->sink) + a->recent > a->budget)
     return bad(SI_E_INVALID, "paged eviction needs a budget of at least sink + recent tokens, and of one");
   if (a->weights_stride == 0 || a->weights_stride >> 44) return bad(SI_E_INVALID, "paged eviction stride is out of range");

@@ -190,7 +190,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const _
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t taken = accepted_of(a, b, lane);
-  if (rank == 0 && threadIdx.x == 0) a.accepted[b] = int32_t(taken);
   Rest r = rest_of(a, b, taken);
   // runs of whole turns, but for the row's end
   const uint32_t turns = (a.vocab + kTurn - 1) / kTurn, runs = size * kWarps;
@@ -223,6 +222,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const _
     if (total > 0.0 || attempt) break;  // the same decision in all CTAs
     cluster_wait();
   }
+  // all CTAs of the cluster have read the count by now: `accepted` may lie over `counts`
+  if (rank == 0 && threadIdx.x == 0) a.accepted[b] = int32_t(taken);
   // A CTA may not leave, nor its totals change, before all have read them.
   if (!(total > 0.0) || rank != owner) {
     if (!(total > 0.0) && rank == 0 && threadIdx.x == 0) a.next[b] = -1;
@@ -274,6 +275,8 @@ int check_verify(const si_verify_drafts* a, std::string* msg) {
   if (!a->target || !a->last_uniform || !a->accepted || !a->next)
     return bad(SI_E_INVALID, "draft verification buffers are null");
   if (a->drafts && (!a->tokens || !a->uniform)) return bad(SI_E_INVALID, "draft verification has no drafts or random numbers");
+  if (!words_aligned({a->target, a->draft, a->tokens, a->counts, a->uniform, a->last_uniform, a->accepted, a->next}))
+    return bad(SI_E_INVALID, "draft verification buffers are not aligned to their elements");
   for (uint64_t s : {a->target_seq_stride, a->target_row_stride, a->draft_seq_stride, a->draft_row_stride})
     if (s >> 44) return bad(SI_E_INVALID, "draft verification strides are out of range");
   const uint64_t need = verify_bytes();

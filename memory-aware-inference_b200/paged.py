@@ -20,11 +20,24 @@ _vp, _u64, _u32, _f32, _f64, _i32 = C.c_void_p, C.c_uint64, C.c_uint32, C.c_floa
 class _Described(C.Structure):
     """A structure that keeps the tensors alive whose addresses it holds."""
 
+    _fits = ()  # (field, value) of the caches that its tensors have the sizes for
+
     def _hold(self, *tensors):
         self._tensors = [t for t in tensors if t is not None]
         at = self._tensors[0].device
         self._device = at.index if at.type == "cuda" else -1
         return self
+
+    def _for(self, kv, *fields):
+        self._fits = tuple((f, getattr(kv, f)) for f in fields)
+        return self
+
+    def check_cache(self, kv):
+        """Refuses a cache that the call's tensors are not made for: another
+        layer's pools of the same shape are fine, other sizes would be read past the end."""
+        for field, n in self._fits:
+            if getattr(kv, field) != n:
+                _fail(f"the call was described for a cache of {field} {n}, not {getattr(kv, field)}")
 
 
 class SiPagedKv(_Described):
@@ -194,6 +207,7 @@ def paged_append(kv: SiPagedKv, q, k, v, q_out, slot, sequence=None, position=No
     a.position = _plain(position, "int32", (n,), "position")
     a.rope = _plain(rope, "int64", (rotary_dim // 2,), "rope") if rotary_dim else None
     _same_device(*given, slot, sequence, position, rope, kv._tensors[0])
+    a._for(kv, "kv_heads", "head_dim")
     return a._hold(*given, slot, sequence, position, rope)
 
 
@@ -225,6 +239,7 @@ def paged_attention(kv: SiPagedKv, q, out, lengths, work, scale: float = 0.0, ls
         _fail("paged attention has weights in and none out")
     a.work, a.work_bytes = _work(work)
     _same_device(q, out, lengths, work, lse, weights_in, weights_out, kv._tensors[0])
+    a._for(kv, "sequences", "kv_heads", "head_dim")
     return a._hold(q, out, lengths, work, lse, weights_in, weights_out)
 
 
@@ -249,6 +264,7 @@ def paged_evict(kv: SiPagedKv, lengths_in, lengths_out, weights_in, weights_out,
     a.positions_out = _plain(positions_out, "int32", shape, "positions_out")
     a.next_position = _plain(next_position, "int32", (n,), "next_position")
     a.work, a.work_bytes = _work(work)
+    a._for(kv, "sequences", "kv_heads")
     held = (lengths_in, lengths_out, weights_in, weights_out, positions_in, positions_out, next_position, work)
     _same_device(*held, kv._tensors[0])
     return a._hold(*held)

@@ -966,3 +966,26 @@ def test_tensors_of_another_device_are_refused(ctx):
         ctx.paged_attention_dev(host, args, LEGACY)
     with pytest.raises(mai.SiError):
         mai.paged_attention(cache.desc, q, q, n, torch.empty(1 << 22, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("n, vocab", [(1, 248320), (9, 32003), (200, 700)])
+def test_accepted_counts_over_the_counts(ctx, n, vocab):
+    """One array for the drafts' counts and the accepted ones, many times: the
+    blocks of a sequence all read the count before it is written over."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    p = torch.softmax(torch.randn(n, 5, vocab, device="cuda", generator=gen), -1)
+    tokens = p[:, :4].argmax(-1).to(torch.int32)
+    u, last = torch.rand(n, 4, device="cuda", generator=gen) * 2e-4, torch.rand(n, device="cuda", generator=gen)
+    counts = torch.randint(0, 5, (n,), device="cuda", generator=gen, dtype=torch.int32)
+    work = torch.empty(16, dtype=torch.uint8, device="cuda")
+    want = run_verify(ctx, p, None, tokens, u, last, counts)
+    following = torch.empty_like(counts)
+    for _ in range(50):
+        both = counts.clone()
+        torch.cuda.synchronize()
+        ctx.verify_drafts_dev(mai.verify_drafts(p, tokens, u, last, both, following, work, counts=both), LEGACY)
+        torch.cuda.synchronize()
+        assert torch.equal(both, want[0]) and torch.equal(following, want[1])
+    for b in range(min(n, 9)):
+        assert (want[0][b].item(), want[1][b].item()) == verified(p[b].cpu().numpy(), None, tokens[b].tolist(), u[b].tolist(),
+                                                                  last[b].item(), int(counts[b]))

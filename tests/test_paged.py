@@ -313,3 +313,46 @@ def test_bindings_refuse_tensors_that_do_not_fit():
         with pytest.raises(mai.SiError):
             f()
             pytest.fail(f"case {i} was taken")
+
+
+WORDS = {"append": ["sequence", "slot", "position"], "attention": ["lengths", "lse", "weights_in", "weights_out"],
+         "evict": ["lengths_in", "lengths_out", "weights_in", "weights_out", "positions_in", "positions_out", "next_position"],
+         "verify": ["target", "draft", "tokens", "counts", "uniform", "last_uniform", "accepted", "next"]}
+
+
+@pytest.mark.parametrize("name, field", [(n, f) for n, fields in WORDS.items() for f in fields])
+def test_misaligned_arrays_are_refused(name, field):
+    make, fn = CALLS[name]
+    args = make(True) if name == "attention" else make()
+    setattr(args[-1], field, (getattr(args[-1], field) or 4096) + 2)
+    refused(fn, *args)
+
+
+@pytest.mark.parametrize("name, other, fits", [
+    ("append", dict(seqs=5), True), ("append", dict(kv_heads=3), False), ("append", dict(hd=24), False),
+    ("attention", dict(), True), ("attention", dict(pages=9, page=16), True), ("attention", dict(seqs=4), False),
+    ("attention", dict(kv_heads=1), False), ("attention", dict(hd=8), False),
+    ("evict", dict(hd=32), True), ("evict", dict(seqs=2), False), ("evict", dict(kv_heads=4), False)])
+def test_a_call_refuses_a_cache_of_other_sizes(name, other, fits):
+    """Another layer's pools of the same shape are the ordinary use."""
+    _, a = CALLS[name][0]()
+    ctx = object.__new__(mai.CudaContext)
+    ctx.device, ctx.h = -1, None  # where tensors on the CPU are; the C call then lacks a context
+    kv = mai.paged_kv(*pools(**other))
+    call = {"append": ctx.paged_append_dev, "attention": ctx.paged_attention_dev, "evict": ctx.paged_evict_dev}[name]
+    if name == "evict":
+        a.work_bytes = 1 << 20  # not read: nothing is launched
+    with pytest.raises(mai.SiError, match="described for a cache" if not fits else "null context"):
+        call(kv, a)
+
+
+def test_outputs_over_inputs_that_others_read_are_refused():
+    kv, a = attention_call()
+    a.out = a.q
+    refused(L.si_paged_attention_dev, kv, a)
+    kv, a = evict_call()
+    other = torch.zeros(3, dtype=torch.int32)
+    a.next_position = a.lengths_out
+    accepted(L.si_paged_evict_dev, kv, a)  # lengths_in too: one array for all three
+    a.lengths_in = other.data_ptr()
+    refused(L.si_paged_evict_dev, kv, a)
