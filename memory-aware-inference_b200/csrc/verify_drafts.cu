@@ -17,10 +17,11 @@
 // finds whose run the draw falls in, and that CTA scans that warp's run
 // again. A difference is max(p - q, 0) = p - min(p, q), so that the minimum is
 // taken in f32 and only the subtraction and the sum in f64. 64 windows over
-// 248,320 tokens take 30 us (107 MB, 3.5 TB/s), one takes 10.5 us.
+// 248,320 tokens take 25 us (107 MB, 4.3 TB/s), one takes 10.5 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -55,24 +56,37 @@ struct Rest {
   }
 };
 
-__device__ __forceinline__ float load_stream(const float* p) {
-  float x;
-  asm volatile("ld.global.nc.L1::no_allocate.f32 %0, [%1];" : "=f"(x) : "l"(p));
-  return x;
+// A lane's tokens of a turn, from the turn's start: 16 bytes at a time where the
+// row is aligned for that (64 windows over 248,320 tokens 28.4 us, 30.6 a token at a time).
+template <bool WIDE>
+__device__ __forceinline__ uint32_t token_of(uint32_t i, uint32_t lane) {
+  return WIDE ? i / 4 * 128 + lane * 4 + i % 4 : i * 32 + lane;
+}
+template <bool WIDE>
+__device__ __forceinline__ void load_turn(float x[kEach], const float* p, uint32_t lane) {
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; i += WIDE ? 4 : 1) {
+    const float* at = p + token_of<WIDE>(i, lane);
+    if constexpr (WIDE)
+      asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(x[i]), "=f"(x[i + 1]), "=f"(x[i + 2]), "=f"(x[i + 3])
+                   : "l"(at));
+    else
+      asm volatile("ld.global.nc.L1::no_allocate.f32 %0, [%1];" : "=f"(x[i]) : "l"(at));
+  }
 }
 
 // Sum of tokens [j0, j1) by one warp, the same in all lanes. All loads of a turn
 // are on their way before the first value is used.
+template <bool WIDE>
 __device__ __forceinline__ double run_sum(const Rest& r, uint32_t j0, uint32_t j1, uint32_t lane) {
   double s = 0.0;
-  uint32_t j = j0 + lane;
-  for (; j - lane + kTurn <= j1; j += kTurn) {
+  uint32_t j = j0;
+  for (; j + kTurn <= j1; j += kTurn) {
     float x[kEach], y[kEach];
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) x[i] = load_stream(r.p + j + i * 32);
+    load_turn<WIDE>(x, r.p + j, lane);
     if (r.q) {
-#pragma unroll
-      for (uint32_t i = 0; i < kEach; ++i) y[i] = load_stream(r.q + j + i * 32);
+      load_turn<WIDE>(y, r.q + j, lane);
 #pragma unroll
       for (uint32_t i = 0; i < kEach; ++i) {
         const float w = weight_of(x[i]);
@@ -80,11 +94,11 @@ __device__ __forceinline__ double run_sum(const Rest& r, uint32_t j0, uint32_t j
       }
     } else {
 #pragma unroll
-      for (uint32_t i = 0; i < kEach; ++i) s += j + i * 32 == r.without ? 0.0 : double(weight_of(x[i]));
+      for (uint32_t i = 0; i < kEach; ++i) s += j + token_of<WIDE>(i, lane) == r.without ? 0.0 : double(weight_of(x[i]));
     }
   }
 #pragma unroll 4
-  for (; j < j1; j += 32) s += r.at(j);
+  for (j += lane; j < j1; j += 32) s += r.at(j);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
@@ -171,12 +185,13 @@ __device__ __forceinline__ uint32_t pick_lane(double weight, double end, double 
   return hit ? __ffs(hit) - 1 : any ? 31 - __clz(any) : 32;
 }
 
-// The lowest index with weight whose end passes the goal, and the highest with
-// weight at all; index rises with the lane, one atomic a warp.
-__device__ __forceinline__ void note_borders(bool weight, bool passes, uint32_t index, uint32_t* pick, uint32_t* last) {
+// The lowest index that passes the goal, and the highest with weight at all;
+// indexes rise with the lane, one atomic a warp.
+__device__ __forceinline__ void note_borders(bool passes, uint32_t passing, bool weight, uint32_t index, uint32_t* pick,
+                                             uint32_t* last) {
   const uint32_t lane = threadIdx.x & 31, any = __ballot_sync(0xffffffffu, weight);
-  const uint32_t hit = __ballot_sync(0xffffffffu, weight && passes);
-  if (hit && lane == uint32_t(__ffs(hit) - 1)) atomicMin(pick, index);
+  const uint32_t hit = __ballot_sync(0xffffffffu, passes);
+  if (hit && lane == uint32_t(__ffs(hit) - 1)) atomicMin(pick, passing);
   if (any && lane == uint32_t(31 - __clz(any))) atomicMax(reinterpret_cast<int*>(last), int(index));
 }
 
@@ -203,7 +218,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const _
       r.without = 0xffffffffu;
     }
     const uint32_t i = rank * kWarps + w;
-    mine = run_sum(r, border(i), border(i + 1), lane);
+    const bool wide = ((reinterpret_cast<uintptr_t>(r.p) | reinterpret_cast<uintptr_t>(r.q)) & 15) == 0;
+    mine = wide ? run_sum<true>(r, border(i), border(i + 1), lane) : run_sum<false>(r, border(i), border(i + 1), lane);
     if (lane == 0) s_run[w] = mine;
     __syncthreads();
     if (w == 0) {
@@ -236,19 +252,42 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const _
   double base = __shfl_sync(0xffffffffu, run_end - run, at & 31);
   const uint32_t j0 = border(rank * kWarps + at), j1 = border(rank * kWarps + at + 1);
   if (threadIdx.x == 0) s_pick = 0xffffffffu, s_last = 0xffffffffu;
-  for (uint32_t j = j0; j < j1; j += THREADS) {  // a token a thread
-    const uint32_t t = j + threadIdx.x;
-    const double x = t < j1 ? r.at(t) : 0.0, in_warp = lane_prefix(x, lane);
-    __syncthreads();
-    if (lane == 31) s_scan[w] = in_warp;
-    __syncthreads();
-    const double ends = lane_prefix(lane < kWarps ? s_scan[lane] : 0.0, lane);
-    const double end = base + (w ? __shfl_sync(0xffffffffu, ends, (w + 31) & 31) : 0.0) + in_warp;
-    note_borders(x > 0.0, end > goal, t, &s_pick, &s_last);
-    base += __shfl_sync(0xffffffffu, ends, 31);
-    __syncthreads();
-    if (s_pick != 0xffffffffu) break;  // the same for all threads
-  }
+  // A step is a chain of scans: long runs take four neighbouring tokens a thread and
+  // step (64 windows over 248,320 tokens 25.7 us, 28.4 a token at a time), short ones
+  // need one step either way (32,003 tokens 8.2 us, 8.7 with four).
+  auto scan = [&](auto tokens) {
+    constexpr uint32_t kScan = decltype(tokens)::value;
+    for (uint32_t j = j0; j < j1; j += kScan * THREADS) {
+      const uint32_t t = j + kScan * threadIdx.x;
+      double x[kScan], sum = 0.0;
+#pragma unroll
+      for (uint32_t i = 0; i < kScan; ++i) x[i] = t + i < j1 ? r.at(t + i) : 0.0;
+#pragma unroll
+      for (uint32_t i = 0; i < kScan; ++i) sum += x[i];
+      const double in_warp = lane_prefix(sum, lane);
+      __syncthreads();
+      if (lane == 31) s_scan[w] = in_warp;
+      __syncthreads();
+      const double ends = lane_prefix(lane < kWarps ? s_scan[lane] : 0.0, lane);
+      const double near = __shfl_up_sync(0xffffffffu, in_warp, 1), far = __shfl_sync(0xffffffffu, ends, (w + 31) & 31);
+      double end = base + (w ? far : 0.0) + (lane ? near : 0.0);
+      uint32_t passing = kScan, last = kScan;  // the first that passes the goal, the last with any weight
+#pragma unroll
+      for (uint32_t i = 0; i < kScan; ++i) {
+        end += x[i];
+        if (x[i] > 0.0) last = i;
+        if (x[i] > 0.0 && end > goal && passing == kScan) passing = i;
+      }
+      note_borders(passing < kScan, t + passing, last < kScan, t + last, &s_pick, &s_last);
+      base += __shfl_sync(0xffffffffu, ends, 31);
+      __syncthreads();
+      if (s_pick != 0xffffffffu) break;  // the same for all threads
+    }
+  };
+  if (j1 - j0 <= THREADS)
+    scan(std::integral_constant<uint32_t, 1>());
+  else
+    scan(std::integral_constant<uint32_t, 4>());
   if (threadIdx.x == 0) a.next[b] = int32_t(s_pick != 0xffffffffu ? s_pick : s_last);
   cluster_wait();
 }

@@ -989,3 +989,23 @@ def test_accepted_counts_over_the_counts(ctx, n, vocab):
     for b in range(min(n, 9)):
         assert (want[0][b].item(), want[1][b].item()) == verified(p[b].cpu().numpy(), None, tokens[b].tolist(), u[b].tolist(),
                                                                   last[b].item(), int(counts[b]))
+
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("n, vocab", [(70, 100000), (90, 100003), (160, 65537)])
+def test_verify_long_runs(ctx, n, vocab, probs):
+    """Enough sequences that a warp's run is longer than its block has threads;
+    rows on and off 16-byte boundaries, most tokens without weight."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    rnd = lambda *s: torch.rand(*s, device="cuda", generator=gen)  # noqa: E731
+    p = torch.where(rnd(n, 2, vocab) < 1e-3, rnd(n, 2, vocab), torch.zeros((), device="cuda"))
+    p /= p.sum(-1, keepdim=True)
+    q = torch.where(rnd(n, 1, vocab) < 0.5, p[:, :1], torch.zeros((), device="cuda")) if probs else None
+    tokens = p[:, :1].argmax(-1).to(torch.int32)
+    u, last = rnd(n, 1), rnd(n)
+    u[::2] = 0.99999
+    last[0], last[1], last[2], last[3] = 0.0, 1 - 2 ** -24, 0.0, 1 - 2 ** -24
+    accepted, following = run_verify(ctx, p, q, tokens, u, last)
+    for b in range(n):
+        want = verified(p[b].cpu().numpy(), q[b].cpu().numpy() if probs else None, tokens[b].tolist(), u[b].tolist(), last[b].item(), 1)
+        assert (accepted[b].item(), following[b].item()) == want, b
