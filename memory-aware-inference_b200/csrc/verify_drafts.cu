@@ -17,7 +17,7 @@
 // finds whose run the draw falls in, and that CTA scans that warp's run
 // again. A difference is max(p - q, 0) = p - min(p, q), so that the minimum is
 // taken in f32 and only the subtraction and the sum in f64. 64 windows over
-// 248,320 tokens take 25 us (107 MB, 4.3 TB/s), one takes 10.5 us.
+// 248,320 tokens take 25 us (107 MB, 4.3 TB/s), one takes 9.5 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -87,11 +87,25 @@ __device__ __forceinline__ double run_sum(const Rest& r, uint32_t j0, uint32_t j
     load_turn<WIDE>(x, r.p + j, lane);
     if (r.q) {
       load_turn<WIDE>(y, r.q + j, lane);
+      // weight_of, but for infinities, which a turn is looked through for at once: one
+      // window of 248,320 tokens 9.5 us, 10.5 with weight_of for each
+      float most = 0.f;
+      double turn = 0.0;
 #pragma unroll
       for (uint32_t i = 0; i < kEach; ++i) {
-        const float w = weight_of(x[i]);
-        s += double(w) - double(fminf(w, weight_of(y[i])));
+        const float w = fmaxf(x[i], 0.f), v = fmaxf(y[i], 0.f);
+        most = fmaxf(most, fmaxf(w, v));
+        turn += double(w) - double(fminf(w, v));
       }
+      if (most == INFINITY) {
+        turn = 0.0;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+          const float w = weight_of(x[i]);
+          turn += double(w) - double(fminf(w, weight_of(y[i])));
+        }
+      }
+      s += turn;
     } else {
 #pragma unroll
       for (uint32_t i = 0; i < kEach; ++i) s += j + token_of<WIDE>(i, lane) == r.without ? 0.0 : double(weight_of(x[i]));

@@ -1009,3 +1009,23 @@ def test_verify_long_runs(ctx, n, vocab, probs):
     for b in range(n):
         want = verified(p[b].cpu().numpy(), q[b].cpu().numpy() if probs else None, tokens[b].tolist(), u[b].tolist(), last[b].item(), 1)
         assert (accepted[b].item(), following[b].item()) == want, b
+
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("n, vocab", [(3, 50000), (3, 50001), (70, 60000)])
+def test_verify_leaves_out_odd_entries_of_long_rows(ctx, n, vocab, probs):
+    """Infinite, NaN and negative entries anywhere in a row, of either side, count as 0."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab + n)
+    p = torch.softmax(torch.randn(n, 2, vocab, device="cuda", generator=gen), -1)
+    q = torch.softmax(torch.randn(n, 1, vocab, device="cuda", generator=gen), -1) if probs else None
+    for side in (p, q):
+        if side is not None:
+            for odd in (math.inf, -math.inf, math.nan, -1.0):
+                at = torch.randint(0, vocab, (n, side.shape[1], 5), device="cuda", generator=gen)
+                side.scatter_(2, at, odd)
+    tokens = torch.randint(0, vocab, (n, 1), device="cuda", generator=gen, dtype=torch.int32)
+    u, last = torch.full((n, 1), 0.999, device="cuda"), torch.linspace(0, 0.999, n, device="cuda")
+    accepted, following = run_verify(ctx, p, q, tokens, u, last)
+    for b in range(n):
+        want = verified(p[b].cpu().numpy(), q[b].cpu().numpy() if probs else None, tokens[b].tolist(), u[b].tolist(), last[b].item(), 1)
+        assert (accepted[b].item(), following[b].item()) == want, b
