@@ -5,12 +5,12 @@
 
 #include <cuda_runtime.h>
 
-#include <atomic>
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
 
 #include "../../include/si_cuda.h"
+#include "raised_limit.h"
 
 namespace si {
 
@@ -129,17 +129,16 @@ __device__ __forceinline__ void scale_min_k4(int index, const uint8_t* s, uint32
 constexpr int kMaxDevices = 64;
 
 // Raise a kernel's dynamic shared memory limit to `bytes` on the current
-// device, once: function attributes belong to a device, so `cache[d]` keeps the
+// device: function attributes belong to a device, so `limits[d]` keeps the
 // limit set so far on device d (a process may drive several devices).
 template <typename F>
-inline cudaError_t raise_smem_limit(F kernel, uint32_t bytes, std::atomic<uint32_t>* cache) {
+inline cudaError_t raise_smem_limit(F kernel, uint32_t bytes, RaisedLimit* limits) {
+  const auto set = [&](uint32_t n) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(n));
+  };
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-  if (cache[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-  if (e == cudaSuccess) cache[dev].store(bytes, std::memory_order_relaxed);
-  return e;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return set(bytes);
+  return limits[dev].raise(bytes, set);
 }
 
 __host__ __device__ constexpr uint32_t block_bytes_of(uint32_t type) {

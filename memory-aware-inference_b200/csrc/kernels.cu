@@ -1152,7 +1152,7 @@ static bool cache_tensor_map(CUtensorMap* map, const void* base, uint32_t hd, ui
 template <int HD, int G>
 static void launch_fa(const CUtensorMap& tk, const CUtensorMap& tv, const AttnArgs& a, cudaLaunchConfig_t cfg,
                       uint32_t nsplit) {
-  static std::atomic<uint32_t> smem_limit[kMaxDevices];  // per instantiation and device
+  static RaisedLimit smem_limit[kMaxDevices];  // per instantiation and device
   constexpr uint32_t smem = FaLayout<HD, G>::bytes;
   raise_smem_limit(attn_split_bf16_kernel<HD, G>, smem, smem_limit);  // a failure shows in the launch
   cfg.gridDim = dim3(nsplit, a.kvh);

@@ -863,9 +863,9 @@ cudaError_t launch(const AttArgs& p, uint32_t grid, cudaStream_t s) {
   constexpr uint32_t kPart = kCols * (HD + 2), kQ = uint32_t(TQ * Sh::kK) * 32 * 4 * Sh::kSplit;
   constexpr uint32_t kRegion = (kQ > kPart ? kQ : kPart) + kPart;
   const uint32_t smem = Sh::kWorkers * kRegion * 4 + (p.kv.sequences + 1) * 4;
-  static std::atomic<uint32_t> cache[kMaxDevices];
+  static RaisedLimit limits[kMaxDevices];
   auto kernel = paged_attention_kernel<HD, BF16, TQ, TP>;
-  if (cudaError_t e = raise_smem_limit(kernel, smem, cache)) return e;
+  if (cudaError_t e = raise_smem_limit(kernel, smem, limits)) return e;
   PdlLaunch l(dim3(grid), dim3(Shape<HD>::kWarps * 32), smem, s);
   if (cudaError_t e = cudaLaunchKernelEx(&l.cfg, kernel, p)) return e;
   if (grid == 1) return cudaSuccess;

@@ -398,9 +398,9 @@ uint64_t evict_bytes(const si_paged_kv& kv) {
 
 template <int THREADS, bool CLUSTER>
 cudaError_t select(const EvictArgs& p, uint32_t rows, uint32_t cluster, uint32_t each, cudaStream_t s) {
-  static std::atomic<uint32_t> cache[kMaxDevices];
+  static RaisedLimit limits[kMaxDevices];
   const uint32_t bytes = (each + THREADS - 1) / THREADS * THREADS * 4;
-  if (cudaError_t e = raise_smem_limit(evict_select_kernel<THREADS, CLUSTER>, bytes, cache)) return e;
+  if (cudaError_t e = raise_smem_limit(evict_select_kernel<THREADS, CLUSTER>, bytes, limits)) return e;
   PdlLaunch l(dim3(rows * cluster), dim3(THREADS), bytes, s);
   if (CLUSTER) l.cluster(cluster);
   return cudaLaunchKernelEx(&l.cfg, evict_select_kernel<THREADS, CLUSTER>, p);

@@ -678,7 +678,7 @@ int launch_qmm_tc(const QmmParams& p, cudaStream_t s, int sm_count, bool pdl, st
             : ti == 1 ? qmm_tc_kernel<SI_GGML_TYPE_Q5_K>
                       : qmm_tc_kernel<SI_GGML_TYPE_Q6_K>;
   if (e == cudaSuccess) {
-    static std::atomic<uint32_t> smem_limit[3][kMaxDevices];  // per type and device
+    static RaisedLimit smem_limit[3][kMaxDevices];  // per type and device
     e = raise_smem_limit(kern, kQtSmemMax, smem_limit[ti]);
   }
   if (e == cudaSuccess) {

@@ -566,7 +566,7 @@ static int launch_qmv_tc_seg(const QmvParams& p, uint32_t seg, int seg2, cudaStr
     uhi = hi;
     ulo = lo;
   }
-  static std::atomic<uint32_t> smem_limit[kMaxDevices];
+  static RaisedLimit smem_limit[kMaxDevices];
   if (cudaError_t e = raise_smem_limit(qmv_tc_kernel, smem, smem_limit)) {
     if (msg) *msg = std::string("cudaFuncSetAttribute(qmv_tc): ") + cudaGetErrorString(e);
     return SI_E_CUDA;

@@ -582,7 +582,7 @@ int launch_qmv_tc6(const QmvParams& p, cudaStream_t stream, int sm_count, bool p
     if (!t6_map(&m0, w, row_bytes / 8, rows, row_bytes, 210, 32)) return SI_E_UNSUPPORTED;
     m1 = m0;
   }
-  static std::atomic<uint32_t> smem_limit[kMaxDevices];
+  static RaisedLimit smem_limit[kMaxDevices];
   if (cudaError_t e = raise_smem_limit(qmv_tc6_kernel, smem, smem_limit)) {
     if (msg) *msg = std::string("cudaFuncSetAttribute(qmv_tc6): ") + cudaGetErrorString(e);
     return SI_E_CUDA;

@@ -356,3 +356,56 @@ def test_outputs_over_inputs_that_others_read_are_refused():
     accepted(L.si_paged_evict_dev, kv, a)  # lengths_in too: one array for all three
     a.lengths_in = other.data_ptr()
     refused(L.si_paged_evict_dev, kv, a)
+
+
+# ---- host state that threads share -----------------------------------------------
+LIMIT_PROGRAM = r"""
+#include "raised_limit.h"
+
+#include <chrono>
+#include <cstdio>
+#include <thread>
+
+static std::atomic<uint32_t> real{0};
+static std::atomic<bool> small_asks{false}, large_set{false}, small_done{false};
+
+static void wait_for(std::atomic<bool>& flag) {  // a fifth of a second at most
+  for (int i = 0; i < 200 && !flag; ++i) std::this_thread::sleep_for(std::chrono::milliseconds(1));
+}
+
+int main() {
+  si::RaisedLimit limit;
+  int calls = 0;
+  // the smaller size asks first, and its attribute call ends after the larger one's if it may
+  std::thread small([&] {
+    limit.raise(100, [&](uint32_t n) { small_asks = true; wait_for(large_set); real = n; return 0; });
+    small_done = true;
+  });
+  std::thread large([&] {
+    wait_for(small_asks);
+    limit.raise(200, [&](uint32_t n) { real = n; large_set = true; wait_for(small_done); return 0; });
+  });
+  small.join();
+  large.join();
+  const auto count = [&](uint32_t n) { ++calls; real = n; return 0; };
+  limit.raise(200, count);
+  if (real < 200 || calls != 0) return std::printf("noted 200, set %u, %d calls\n", real.load(), calls), 1;
+  limit.raise(150, count);
+  if (real != 200 || calls != 0) return std::printf("lowered\n"), 2;
+  // a refused size is not noted
+  if (limit.raise(300, [&](uint32_t) { return 7; }) != 7) return 3;
+  limit.raise(300, count);
+  return real == 300 && calls == 1 ? 0 : 4;
+}
+"""
+
+
+def test_a_raised_limit_is_never_lowered_by_another_thread(tmp_path):
+    """Two threads raise one kernel's limit to different sizes at once."""
+    import subprocess
+    src, exe = tmp_path / "limit.cpp", tmp_path / "limit"
+    src.write_text(LIMIT_PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-pthread", "-I",
+                    os.path.join(REPO, "memory-aware-inference_b200", "csrc"), str(src), "-o", str(exe)], check=True)
+    got = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert got.returncode == 0, (got.returncode, got.stdout)
