@@ -22,8 +22,9 @@
  * Errors found on the device (a page number outside the pool, a length beyond
  * the page table or the weights' rows, a drafted token outside the vocabulary)
  * neither read nor write out of bounds: the offending token is left out, and
- * the context's next si_ctx_synchronize or host-memory call that follows the
- * work's end returns SI_E_INVALID for it.
+ * si_ctx_synchronize or a host-memory call of the context returns SI_E_INVALID
+ * for it, once: the first that finds it, at the latest the first that follows
+ * the work's end.
  *
  * Calls that overlap on the GPU need workspaces of their own, and so do CUDA
  * graphs that may be replayed at the same time.

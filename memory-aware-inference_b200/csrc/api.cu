@@ -110,6 +110,23 @@ void note_weights(si_ctx* ctx, int64_t delta) {
   }
 }
 
+// Bits may be set at any time by a kernel on another stream, so the word is read
+// and cleared in one step; word[1] gets what it held.
+__global__ void take_error_kernel(int* word) { word[1] = atomicExch(word, 0); }
+
+// The error bits, taken. On the context's own stream: on the legacy stream it
+// would wait for other work there, and with it take that work's bits.
+static cudaError_t take_error(si_ctx* ctx, int* bits) {
+  cudaError_t e = cudaSetDevice(ctx->device);
+  if (e != cudaSuccess) return e;
+  take_error_kernel<<<1, 1, 0, ctx->stream>>>(ctx->d_err);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  e = cudaMemcpyAsync(ctx->h_err, ctx->d_err + 1, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+  if (e == cudaSuccess) *bits = *ctx->h_err;
+  return e;
+}
+
 int sync_and_check(si_ctx* ctx, const char* what) {
   auto t0 = std::chrono::steady_clock::now();
   ctx->submitted++;
@@ -125,13 +142,11 @@ int sync_and_check(si_ctx* ctx, const char* what) {
   ctx->pending.clear();
   ctx->h_stage_used = 0;
   if (e != cudaSuccess) return cuda_fail(ctx, e, what);
-  const int bits = *ctx->h_err;
-  if (bits) {
-    cudaMemset(ctx->d_err, 0, sizeof(int));
+  if (int bits = *ctx->h_err) {
+    if ((e = take_error(ctx, &bits)) != cudaSuccess) return cuda_fail(ctx, e, what);
     const bool gave_up = bits & (KERR_TIMEOUT_FULL | KERR_TIMEOUT_EMPTY | KERR_TIMEOUT_DRAIN);
     // a kernel that gave up may have left split-group counters behind
     if (gave_up && ctx->qscratch.p) cudaMemset(ctx->qscratch.p, 0, ctx->qscratch.cap);
-    *ctx->h_err = 0;
     if (!gave_up && bits == KERR_BAD_INDEX)  // a value that the caller passed in device memory
       return fail(ctx, SI_E_INVALID, std::string(what) + ": a page, length, slot or token is out of range");
     return fail(ctx, gave_up ? SI_E_TIMEOUT : SI_E_CUDA,
@@ -246,6 +261,13 @@ int si_ctx_create(int device, const si_ctx_config* cfg, si_ctx** out) {
     return rc;
   }
   cudaMemset(c->d_err, 0, 64);
+  // loaded now: a kernel loaded at its first launch may wait for work on other streams
+  cudaFuncAttributes attributes;
+  if ((e = cudaFuncGetAttributes(&attributes, take_error_kernel)) != cudaSuccess) {
+    int rc = cuda_fail(nullptr, e, "context creation");
+    si_ctx_destroy(c);
+    return rc;
+  }
   cudaMemset(c->d_argmax, 0, 64);
   cudaDeviceSynchronize();
   *out = c;

@@ -1029,3 +1029,30 @@ def test_verify_leaves_out_odd_entries_of_long_rows(ctx, n, vocab, probs):
     for b in range(n):
         want = verified(p[b].cpu().numpy(), q[b].cpu().numpy() if probs else None, tokens[b].tolist(), u[b].tolist(), last[b].item(), 1)
         assert (accepted[b].item(), following[b].item()) == want, b
+
+
+def test_a_report_on_another_stream_is_not_lost(ctx):
+    """The context's stream and the legacy one each hold a call with a bad slot, the legacy one's behind some
+    work. Reporting the first must not clear the second, which is not there yet."""
+    cache = Cache([16], 1, 8, 64, BF16, seed=2)
+    new = torch.zeros(1, 1, 64, dtype=BF16, device="cuda")
+    slot = torch.tensor([16], dtype=torch.int32, device="cuda")  # beyond the table
+    bad = mai.paged_append(cache.desc, None, new, new, None, slot)
+    for stream in (None, LEGACY):  # both kinds of launch once, so that nothing is loaded below
+        ctx.paged_append_dev(cache.desc, bad, stream)
+        torch.cuda.synchronize()
+        with pytest.raises(mai.SiError):
+            ctx.synchronize()
+    ctx.synchronize()
+    torch.cuda._sleep(200_000_000)  # about a tenth of a second
+    ctx.paged_append_dev(cache.desc, bad, LEGACY)
+    ctx.paged_append_dev(cache.desc, bad, None)
+    with pytest.raises(mai.SiError) as e:
+        ctx.synchronize()
+    assert e.value.status == mai.SI_E_INVALID
+    assert not torch.cuda.default_stream().query()  # the other call is still to come
+    torch.cuda.synchronize()
+    with pytest.raises(mai.SiError) as e:
+        ctx.synchronize()
+    assert e.value.status == mai.SI_E_INVALID
+    ctx.synchronize()
