@@ -106,7 +106,11 @@ int si_rope_table(double theta, uint32_t rotary_dim, const si_rope_scaling* scal
  * sequence[t]. A token whose slot is negative is padding: nothing of it is
  * written, neither cache nor q_out. Two tokens of a call must not share a
  * (sequence, slot). q and q_out may be the same memory with the same strides.
- * Strides count elements; dims are contiguous. */
+ * Strides count elements; dims are contiguous.
+ * With weights and positions, the arrays that attention adds to and eviction
+ * reads, every appended slot starts with weight 0 and its token's position in
+ * each kv head. A slot behind a cut holds what the token that left it had
+ * gathered, so a cache that is evicted from needs this with every append. */
 typedef struct si_paged_append {
   const void* q;            /* [tokens][query_heads][head_dim]; NULL: none */
   void* q_out;
@@ -122,6 +126,9 @@ typedef struct si_paged_append {
   uint32_t elem;            /* type of q, k, v and q_out: SI_ELEM_* */
   uint32_t tokens;          /* 0: nothing to do */
   uint32_t query_heads, rotary_dim, rope_layout;
+  float* weights;           /* [sequences][kv_heads][weights_stride]; NULL: not wanted. Needs k and v */
+  int32_t* positions;       /* the same */
+  uint64_t weights_stride;  /* of both, entries; a slot at or beyond it is out of range */
 } si_paged_append;
 int si_paged_append_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_append* a, void* stream);
 
@@ -164,7 +171,10 @@ int si_paged_attention_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_at
  * weight leave, of equal ones the lowest slot first (NaN counts as smaller
  * than any number). Kept tokens of slots >= budget move into the slots that
  * became free below it, both in order; nothing else moves. Attention does not
- * depend on the order of slots: keys carry their position. The pages that hold
+ * depend on the order of slots: keys carry their position, and from the first
+ * cut on a slot's number is not its token's position any more: positions and
+ * next_position are then needed, and every append has to start its slots'
+ * weights and positions anew (si_paged_append). The pages that hold
  * no slot below the new length can be given to other sequences afterwards.
  * Should more than `budget` tokens be protected (positions that repeat),
  * the protected ones of the lowest slots leave, after all others.

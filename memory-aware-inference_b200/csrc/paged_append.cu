@@ -30,6 +30,9 @@ struct AppendArgs {
   uint32_t rot_parts;    // parts of a head that rotate
   FastDiv parts;         // parts of a head, a thread each
   FastDiv q_heads, kv_heads;
+  float* weights;        // accumulated weights and positions that appended slots start anew in; may be null
+  int32_t* positions;
+  uint64_t weights_stride;
   int* err;
 };
 
@@ -87,6 +90,7 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const __grid_consta
   extern __shared__ float2 s_turn[];  // [per_cta][VEC][rotating parts] (cos, sin)
   __shared__ uint64_t s_cell[kMaxTokens];
   __shared__ int32_t s_slot[kMaxTokens];
+  __shared__ uint32_t s_seq[kMaxTokens];
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t t0 = blockIdx.x * a.per_cta, nt = min(a.per_cta, a.tokens - t0);
@@ -96,7 +100,8 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const __grid_consta
     uint64_t cell = kNoCell;
     if (slot >= 0 && a.kvh) {
       const uint32_t b = a.sequence ? uint32_t(a.sequence[tok]) : tok;
-      if (b < a.kv.sequences && uint32_t(slot) < a.kv.max_tokens)
+      s_seq[threadIdx.x] = b;
+      if (b < a.kv.sequences && uint32_t(slot) < a.kv.max_tokens && uint32_t(slot) < a.weights_stride)
         cell = paged_slot(a.kv, a.kv.pages + b * a.kv.pages_stride, uint32_t(slot), 0);
       if (cell == kNoCell) atomicOr(a.err, KERR_BAD_INDEX);
     }
@@ -114,6 +119,15 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const __grid_consta
     s_turn[t * a.half + j % VEC * a.rot_parts + j / VEC] = make_float2(c * a.rope_scale, s * a.rope_scale);
   }
   __syncthreads();
+  if (a.weights || a.positions) {
+    for (uint32_t i = threadIdx.x; i < nt * a.kvh; i += kThreads) {
+      const uint32_t t = div_of(i, a.kv_heads), h = i - t * a.kvh;
+      if (s_cell[t] == kNoCell) continue;
+      const uint64_t at = (uint64_t(s_seq[t]) * a.kvh + h) * a.weights_stride + uint32_t(s_slot[t]);
+      if (a.weights) a.weights[at] = 0.f;
+      if (a.positions) a.positions[at] = a.position ? a.position[t0 + t] : s_slot[t];
+    }
+  }
   const uint32_t row0 = div_of(threadIdx.x, a.parts), part = threadIdx.x - row0 * a.parts.d, rows_at_once = kThreads / a.parts.d;
   if (row0 >= rows_at_once) return;
   const bool rotates = part < a.rot_parts;
@@ -227,8 +241,13 @@ int check_append(const si_paged_kv* kv, const si_paged_append* a, std::string* m
     return bad(SI_E_INVALID, "paged append has more tokens than sequences and no sequence numbers");
   for (const void* p : {a->q, static_cast<const void*>(a->q_out), a->k, a->v})
     if (!elem_aligned(p, a->elem)) return bad(SI_E_INVALID, "paged append buffers are not aligned to their elements");
-  if (!words_aligned({a->sequence, a->slot, a->position}))
+  if (!words_aligned({a->sequence, a->slot, a->position, a->weights, a->positions}))
     return bad(SI_E_INVALID, "paged append arrays of 32-bit numbers are not aligned");
+  if (a->weights || a->positions) {
+    if (a->tokens && !a->k) return bad(SI_E_INVALID, "paged append starts weights and positions of appended keys only");
+    if (a->weights_stride == 0 || a->weights_stride >> 44)
+      return bad(SI_E_INVALID, "paged append stride of weights and positions is out of range");
+  }
   const uint64_t strides[] = {a->q_token_stride,     a->q_head_stride, a->q_out_token_stride, a->q_out_head_stride,
                               a->k_token_stride,     a->k_head_stride, a->v_token_stride,     a->v_head_stride};
   for (uint64_t s : strides)
@@ -263,6 +282,8 @@ extern "C" int si_paged_append_dev(si_ctx* ctx, const si_paged_kv* kv, const si_
   p.kvh = a->k ? kv->kv_heads : 0;
   p.half = a->rotary_dim / 2;
   p.interleaved = a->rope_layout == SI_ROPE_INTERLEAVED;
+  p.weights = a->weights, p.positions = a->positions;
+  p.weights_stride = a->weights || a->positions ? a->weights_stride : ~uint64_t(0);
   p.err = ctx->d_err;
   // 16-byte accesses where every run starts on a 16-byte boundary
   bool wide = p.interleaved ? a->rotary_dim % 16 == 0 : p.half % 8 == 0;

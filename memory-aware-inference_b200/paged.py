@@ -56,7 +56,8 @@ class SiPagedAppend(_Described):
                 ("q_out_token_stride", _u64), ("q_out_head_stride", _u64), ("k_token_stride", _u64),
                 ("k_head_stride", _u64), ("v_token_stride", _u64), ("v_head_stride", _u64), ("sequence", _vp),
                 ("slot", _vp), ("position", _vp), ("rope", _vp), ("rope_scale", _f32), ("elem", _u32), ("tokens", _u32),
-                ("query_heads", _u32), ("rotary_dim", _u32), ("rope_layout", _u32)]
+                ("query_heads", _u32), ("rotary_dim", _u32), ("rope_layout", _u32), ("weights", _vp),
+                ("positions", _vp), ("weights_stride", _u64)]
 
 
 class SiPagedAttention(_Described):
@@ -175,11 +176,12 @@ def rope_table(theta: float, rotary_dim: int, kind: str = "none", factor: float 
 
 
 def paged_append(kv: SiPagedKv, q, k, v, q_out, slot, sequence=None, position=None, rope=None, rotary_dim: int = 0,
-                 layout: str = "interleaved", rope_scale: float = 1.0) -> SiPagedAppend:
+                 layout: str = "interleaved", rope_scale: float = 1.0, weights=None, positions=None) -> SiPagedAppend:
     """si_paged_append: q [tokens][query_heads][head_dim] with q_out, k and v
     [tokens][kv_heads][head_dim] (either pair may be None), slot, sequence and
     position int32 [tokens], rope the device copy of `rope_table`'s turns
-    (int64 [rotary_dim / 2])."""
+    (int64 [rotary_dim / 2]); weights float32 and positions int32
+    [sequences][kv_heads][slots], where appended slots start anew."""
     if layout not in _LAYOUTS:
         _fail(f"unknown rotary layout {layout!r}")
     if slot.dim() != 1:
@@ -206,9 +208,15 @@ def paged_append(kv: SiPagedKv, q, k, v, q_out, slot, sequence=None, position=No
     a.sequence = _plain(sequence, "int32", (n,), "sequence")
     a.position = _plain(position, "int32", (n,), "position")
     a.rope = _plain(rope, "int64", (rotary_dim // 2,), "rope") if rotary_dim else None
-    _same_device(*given, slot, sequence, position, rope, kv._tensors[0])
-    a._for(kv, "kv_heads", "head_dim")
-    return a._hold(*given, slot, sequence, position, rope)
+    started = [t for t in (weights, positions) if t is not None]
+    if started:
+        shape = (kv.sequences, kv.kv_heads, started[0].shape[-1])
+        a.weights = _plain(weights, "float32", shape, "weights")
+        a.positions = _plain(positions, "int32", shape, "positions")
+        a.weights_stride = shape[2]
+    _same_device(*given, slot, sequence, position, rope, *started, kv._tensors[0])
+    a._for(kv, "kv_heads", "head_dim", *(("sequences",) if started else ()))
+    return a._hold(*given, slot, sequence, position, rope, *started)
 
 
 def paged_attention_workspace_bytes(kv: SiPagedKv, query_heads: int, weights: bool = False) -> int:

@@ -1056,3 +1056,78 @@ def test_a_report_on_another_stream_is_not_lost(ctx):
         ctx.synchronize()
     assert e.value.status == mai.SI_E_INVALID
     ctx.synchronize()
+
+
+def test_slots_behind_a_cut_start_anew(ctx):
+    """The serving loop over arrays that hold other tokens' weights and positions at every slot not in use:
+    whatever lies there, a new token's weight counts from 0 and its position is its own."""
+    kvh, g, hd, budget, sink, recent, seqs = 2, 2, 64, 20, 2, 4, 3
+    gen = torch.Generator().manual_seed(5)
+    cache = Cache([0] * seqs, kvh, 8, hd, BF16, seed=6, room=4)
+    weights = torch.full((seqs, kvh, 32), 7e3, device="cuda")  # would outweigh every real one
+    positions = torch.full((seqs, kvh, 32), -5, dtype=torch.int32, device="cuda")  # would be protected
+    length, seen = torch.zeros(seqs, dtype=torch.int32, device="cuda"), [0] * seqs
+    attention_work, evict_work = work_for(cache, kvh * g, True), torch.empty(mai.paged_evict_workspace_bytes(cache.desc),
+                                                                             dtype=torch.uint8, device="cuda")
+    want_w, want_p = [[{} for _ in range(kvh)] for _ in range(seqs)], [[{} for _ in range(kvh)] for _ in range(seqs)]
+    for step in range(12):
+        rows = [(b, length[b].item() + i, seen[b] + i) for b in range(seqs) for i in range((4, 1, 3)[(b + step) % 3])]
+        sequence, slot, position = (torch.tensor(x, dtype=torch.int32).cuda() for x in zip(*rows))
+        k, v = (torch.randn(len(rows), kvh, hd, generator=gen).to(BF16).cuda() for _ in range(2))
+        ctx.paged_append_dev(cache.desc, mai.paged_append(cache.desc, None, k, v, None, slot, sequence=sequence, position=position,
+                                                          weights=weights, positions=positions), LEGACY)
+        for b, t, p in rows:
+            seen[b] = p + 1
+            length[b] = t + 1
+            for h in range(kvh):
+                want_w[b][h][t], want_p[b][h][t] = 0.0, p
+        q = torch.randn(seqs, kvh * g, hd, generator=gen).cuda()
+        out = torch.empty_like(q)
+        ctx.paged_attention_dev(cache.desc, mai.paged_attention(cache.desc, q, out, length, attention_work, weights_in=weights,
+                                                                weights_out=weights), LEGACY)
+        want, _, probs = reference(cache, q, lengths=length.tolist())
+        close(out, want, F32)
+        before = weights.clone()
+        for b in range(seqs):
+            for h in range(kvh):
+                for t in range(length[b].item()):
+                    want_w[b][h][t] += probs[b][h, t].item()
+                    assert before[b, h, t].item() == pytest.approx(want_w[b][h][t], rel=1e-5, abs=1e-6)
+        nxt = torch.tensor(seen, dtype=torch.int32, device="cuda")
+        n = length.tolist()
+        ctx.paged_evict_dev(cache.desc, mai.paged_evict(cache.desc, length, length, weights, weights, budget, evict_work, sink=sink,
+                                                        recent=recent, positions_in=positions, positions_out=positions,
+                                                        next_position=nxt), LEGACY)
+        assert length.tolist() == [min(x, budget) for x in n]
+        for b in range(seqs):
+            for h in range(kvh):
+                of = [want_p[b][h][t] for t in range(n[b])]
+                holes, movers = evicted(before[b, h].tolist(), of, n[b], budget, sink, recent, seen[b])
+                for a, c in zip(holes, movers):
+                    want_w[b][h][a], want_p[b][h][a] = want_w[b][h][c], want_p[b][h][c]
+                assert positions[b, h, :length[b]].tolist() == [want_p[b][h][t] for t in range(length[b].item())]
+    ctx.synchronize()
+
+
+def test_append_leaves_out_slots_beyond_the_started_arrays(ctx):
+    """Slots that the weights have no entry for are reported, and nothing of the token is written."""
+    cache = Cache([32, 32], 2, 8, 64, BF16, seed=3)
+    k0 = cache.k.clone()
+    weights = torch.full((2, 2, 20), 3.0, device="cuda")
+    positions = torch.full((2, 2, 20), 9, dtype=torch.int32, device="cuda")
+    new = torch.randn(4, 2, 64, device="cuda").to(BF16)
+    slot = torch.tensor([20, 19, -1, 31], dtype=torch.int32, device="cuda")
+    sequence = torch.tensor([0, 1, 1, 1], dtype=torch.int32, device="cuda")
+    ctx.paged_append_dev(cache.desc, mai.paged_append(cache.desc, None, new, new, None, slot, sequence=sequence, weights=weights,
+                                                      positions=positions), LEGACY)
+    torch.cuda.synchronize()
+    with pytest.raises(mai.SiError) as e:
+        ctx.synchronize()
+    assert e.value.status == mai.SI_E_INVALID
+    assert (weights[1, :, 19] == 0).all() and (positions[1, :, 19] == 19).all()
+    weights[1, :, 19], positions[1, :, 19] = 3.0, 9
+    assert (weights == 3).all() and (positions == 9).all()
+    pg = cache.pages[1, 2].item()
+    assert torch.equal(cache.k[pg, :, 3], new[1])
+    cache.k[pg, :, 3] = k0[pg, :, 3]
+    assert torch.equal(cache.k.view(torch.int16), k0.view(torch.int16))

@@ -409,3 +409,32 @@ def test_a_raised_limit_is_never_lowered_by_another_thread(tmp_path):
                     os.path.join(REPO, "memory-aware-inference_b200", "csrc"), str(src), "-o", str(exe)], check=True)
     got = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert got.returncode == 0, (got.returncode, got.stdout)
+
+
+@pytest.mark.parametrize("field", ["weights", "positions"])
+def test_started_arrays_of_an_append(field):
+    """Weights and positions that an append starts anew: with keys, a stride and whole words only."""
+    def call():
+        kv, a = append_call()
+        setattr(a, field, 4096)
+        a.weights_stride = 8
+        return kv, a
+    kv, a = call()
+    accepted(L.si_paged_append_dev, kv, a)
+    for change in (dict(k=None, v=None), dict(weights_stride=0), dict(weights_stride=1 << 44), {field: 4098}):
+        kv, a = call()
+        for name, value in change.items():
+            setattr(a, name, value)
+        refused(L.si_paged_append_dev, kv, a)
+    kv = mai.paged_kv(*pools())
+    n, k = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 2, 16)
+    made = mai.paged_append(kv, None, k, k, None, n, weights=torch.zeros(3, 2, 8), positions=torch.zeros(3, 2, 8, dtype=torch.int32))
+    assert made.weights_stride == 8 and made.weights and made.positions
+    for wrong in (dict(weights=torch.zeros(3, 2, 8).double()), dict(weights=torch.zeros(2, 2, 8)), dict(positions=torch.zeros(3, 2, 8)),
+                  dict(weights=torch.zeros(3, 2, 8), positions=torch.zeros(3, 2, 9, dtype=torch.int32))):
+        with pytest.raises(mai.SiError):
+            mai.paged_append(kv, None, k, k, None, n, **wrong)
+    ctx = object.__new__(mai.CudaContext)
+    ctx.device, ctx.h = -1, None
+    with pytest.raises(mai.SiError, match="described for a cache"):
+        ctx.paged_append_dev(mai.paged_kv(*pools(seqs=5)), made)
