@@ -1131,3 +1131,27 @@ def test_append_leaves_out_slots_beyond_the_started_arrays(ctx):
     assert torch.equal(cache.k[pg, :, 3], new[1])
     cache.k[pg, :, 3] = k0[pg, :, 3]
     assert torch.equal(cache.k.view(torch.int16), k0.view(torch.int16))
+
+
+def test_attention_long_rows_are_not_biased(ctx):
+    """Positive values over rows of 131,072 slots that one worker walks whole: sums that are cut off, not rounded,
+    fall short by half a unit in the last place an addition, a few 1e-4 here. Roundings of either sign leave the
+    mean error of all outputs far below one output's: half a step / sqrt(3 N) with N outputs, were they independent;
+    a sixteenth of half a step (3e-5) leaves room for outputs of a dim that lie close together."""
+    n, hd, page = 131072, 64, 256
+    rows = min(4096, 24 * torch.cuda.get_device_properties(0).multi_processor_count)  # two for each worker of 12 a multiprocessor
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    k = torch.randn(n // page, 1, page, hd, device="cuda", generator=gen).to(F16)
+    v = ((0.5 + torch.rand(n // page, 1, page, hd, device="cuda", generator=gen)) *
+         (1 + torch.rand(hd, device="cuda", generator=gen))).to(F16)
+    pages = torch.arange(n // page, dtype=torch.int32, device="cuda").expand(rows, -1).contiguous()
+    kv = mai.paged_kv(k, v, pages)
+    q = torch.randn(rows, 1, hd, device="cuda", generator=gen).to(F16)
+    out, length = torch.empty_like(q), torch.full((rows,), n, dtype=torch.int32, device="cuda")
+    work = torch.empty(mai.paged_attention_workspace_bytes(kv, 1), dtype=torch.uint8, device="cuda")
+    ctx.paged_attention_dev(kv, mai.paged_attention(kv, q, out, length, work), LEGACY)
+    keys, values = (x.reshape(n, hd).double() for x in (k, v))
+    want = torch.cat([torch.softmax(x.double() @ keys.T / hd ** 0.5, -1) @ values for x in q[:, 0].split(256)])
+    error = (out[:, 0].double() - want) / want
+    assert error.abs().max() <= half_step(F16) * 1.02  # the rounding itself, and 2e-2 of it for all sums
+    assert abs(error.mean().item()) <= half_step(F16) / 16
