@@ -96,14 +96,17 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const __grid_consta
   const uint32_t t0 = blockIdx.x * a.per_cta, nt = min(a.per_cta, a.tokens - t0);
   if (threadIdx.x < nt) {
     const uint32_t tok = t0 + threadIdx.x;
-    const int32_t slot = a.slot[tok];
+    int32_t slot = a.slot[tok];
     uint64_t cell = kNoCell;
     if (slot >= 0 && a.kvh) {
       const uint32_t b = a.sequence ? uint32_t(a.sequence[tok]) : tok;
       s_seq[threadIdx.x] = b;
       if (b < a.kv.sequences && uint32_t(slot) < a.kv.max_tokens && uint32_t(slot) < a.weights_stride)
         cell = paged_slot(a.kv, a.kv.pages + b * a.kv.pages_stride, uint32_t(slot), 0);
-      if (cell == kNoCell) atomicOr(a.err, KERR_BAD_INDEX);
+      if (cell == kNoCell) {  // reported, and left out like padding
+        atomicOr(a.err, KERR_BAD_INDEX);
+        slot = -1;
+      }
     }
     s_slot[threadIdx.x] = slot;
     s_cell[threadIdx.x] = cell;

@@ -1155,3 +1155,18 @@ def test_attention_long_rows_are_not_biased(ctx):
     error = (out[:, 0].double() - want) / want
     assert error.abs().max() <= half_step(F16) * 1.02  # the rounding itself, and 2e-2 of it for all sums
     assert abs(error.mean().item()) <= half_step(F16) / 16
+
+
+def test_append_leaves_out_the_queries_of_bad_tokens(ctx):
+    """A token whose slot, sequence or page does not exist is left out whole: its queries are not written either."""
+    cache = Cache([16, 16], 2, 8, 64, BF16, seed=4)
+    cache.pages_dev[1, 1] = -3
+    slot = torch.tensor([3, 16, 9, 2, 5], dtype=torch.int32, device="cuda")
+    sequence = torch.tensor([0, 0, 1, -1, 1], dtype=torch.int32, device="cuda")
+    q, k = torch.randn(5, 4, 64, device="cuda"), torch.randn(5, 2, 64, device="cuda")
+    out = torch.full_like(q, 7.0)
+    ctx.paged_append_dev(cache.desc, mai.paged_append(cache.desc, q, k, k, out, slot, sequence=sequence), LEGACY)
+    torch.cuda.synchronize()
+    with pytest.raises(mai.SiError):
+        ctx.synchronize()
+    assert torch.equal(out[[0, 4]], q[[0, 4]]) and (out[1:4] == 7).all()
