@@ -147,7 +147,7 @@ int si_paged_append_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_appen
  * weights_out, or NULL for zeros. */
 typedef struct si_paged_attention {
   const void* q;            /* [sequences][query_heads][head_dim] */
-  void* out;                /* not q: several blocks read a query */
+  void* out;                /* no element of q: several blocks read a query; rows apart from each other */
   uint64_t q_seq_stride, q_head_stride, out_seq_stride, out_head_stride;
   const int32_t* lengths;   /* [sequences], each at most max_pages * page_tokens */
   float scale;              /* 0: 1 / sqrt(head_dim) */

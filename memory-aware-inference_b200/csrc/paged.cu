@@ -1,5 +1,6 @@
 // Host side of the paged cache: checks of its description, the place of a
 // slot, and the table of rotary frequencies (include/si_paged.h).
+#include <algorithm>
 #include <cmath>
 
 #include "paged.cuh"
@@ -39,6 +40,58 @@ int check_paged_kv(const si_paged_kv* kv, std::string* msg) {
       reinterpret_cast<uintptr_t>(kv->pages) % 4)
     return bad(SI_E_INVALID, "paged cache pools must be 16-byte aligned");
   return SI_OK;
+}
+
+namespace {
+using wide = __int128;
+
+struct Axis {
+  uint64_t n, stride;
+};
+bool distinct(std::initializer_list<Axis> given, uint32_t dims) {
+  Axis axes[3];
+  int count = 0;
+  for (const Axis& a : given)
+    if (a.n > 1) axes[count++] = a;
+  std::sort(axes, axes + count, [](const Axis& a, const Axis& b) { return a.stride < b.stride; });
+  wide span = dims;
+  for (int i = 0; i < count; ++i) {
+    if (wide(axes[i].stride) < span) return false;
+    span += wide(axes[i].n - 1) * axes[i].stride;
+  }
+  return true;
+}
+// Bytes from the first element to behind the last.
+wide span_of(const BufferRows& r) {
+  return (wide(r.n0 - 1) * r.s0 + wide(r.n1 - 1) * r.s1 + r.dims) * elem_bytes(r.elem);
+}
+}  // namespace
+
+bool rows_distinct(const BufferRows& r) { return distinct({{r.n0, r.s0}, {r.n1, r.s1}}, r.dims); }
+
+bool rows_meet(const BufferRows& a, const BufferRows& b) {
+  const wide apart = wide(reinterpret_cast<uintptr_t>(b.p)) - wide(reinterpret_cast<uintptr_t>(a.p));
+  if (apart >= span_of(a) || -apart >= span_of(b)) return false;
+  // an axis of one row has no stride of its own
+  if ((a.n0 > 1 && b.n0 > 1 && a.s0 != b.s0) || (a.n1 > 1 && b.n1 > 1 && a.s1 != b.s1)) return true;
+  const wide s0 = a.n0 > 1 ? a.s0 : b.s0, s1 = a.n1 > 1 ? a.s1 : b.s1, elem = elem_bytes(a.elem);
+  // Rows (i0, i1) of a and (j0, j1) of b share an element if |apart - (i0 - j0) s0 -
+  // (i1 - j1) s1| < dims. The shorter axis is walked, the nearest step of the other computed.
+  struct Steps {
+    wide lo, hi, stride;
+  } x = {-wide(b.n0 - 1), wide(a.n0 - 1), s0}, y = {-wide(b.n1 - 1), wide(a.n1 - 1), s1};
+  if (x.hi - x.lo < y.hi - y.lo) std::swap(x, y);
+  const wide dims = wide(a.dims) * elem;
+  for (wide i = y.lo; i <= y.hi; ++i) {
+    const wide rest = apart - i * y.stride * elem;
+    wide near = x.stride ? rest / (x.stride * elem) : 0;
+    for (wide k : {near - 1, near, near + 1}) {
+      k = std::min(std::max(k, x.lo), x.hi);
+      const wide left = rest - k * x.stride * elem;
+      if (left > -dims && left < dims) return true;
+    }
+  }
+  return false;
 }
 
 }  // namespace si

@@ -168,6 +168,20 @@ inline bool words_aligned(std::initializer_list<const void*> arrays) {
     if (reinterpret_cast<uintptr_t>(p) % 4) return false;
   return true;
 }
+// Rows of a call's buffer: [n0][n1][dims], strides and dims in elements.
+struct BufferRows {
+  const void* p;
+  uint64_t n0, s0, n1, s1;
+  uint32_t dims, elem;
+};
+// Whether no element belongs to two rows: every axis steps over all that the
+// axes of smaller strides span. (Rows that interleave in no such order count as
+// shared; views of one allocation do not.)
+bool rows_distinct(const BufferRows& r);
+// Whether any element is in both buffers, of one element type. Exact where the
+// strides are the same (parts of one buffer); otherwise buffers whose ranges
+// overlap count as sharing.
+bool rows_meet(const BufferRows& a, const BufferRows& b);
 inline bool elem_known(uint32_t elem) { return elem <= SI_ELEM_F16; }
 
 // Makes the context's device current for the launches of one call.

@@ -837,7 +837,6 @@ int check_attention(const si_paged_kv* kv, const si_paged_attention* a, std::str
   if (int rc = check_heads(kv, a->query_heads, msg)) return rc;
   if (!elem_known(a->elem)) return bad(SI_E_UNSUPPORTED, "paged attention elements must be f32, bf16 or f16");
   if (!a->q || !a->out || !a->lengths) return bad(SI_E_INVALID, "paged attention buffers are null");
-  if (a->q == a->out) return bad(SI_E_INVALID, "paged attention cannot write its output over the queries");
   if (!elem_aligned(a->q, a->elem) || !elem_aligned(a->out, a->elem) ||
       !words_aligned({a->lengths, a->lse, a->weights_in, a->weights_out}))
     return bad(SI_E_INVALID, "paged attention buffers are not aligned to their elements");
@@ -845,6 +844,10 @@ int check_attention(const si_paged_kv* kv, const si_paged_attention* a, std::str
   if (a->weights_in && !a->weights_out) return bad(SI_E_INVALID, "paged attention has weights in and none out");
   for (uint64_t s : {a->q_seq_stride, a->q_head_stride, a->out_seq_stride, a->out_head_stride, a->weights_stride})
     if (s >> 44) return bad(SI_E_INVALID, "paged attention strides are out of range");
+  const BufferRows q = {a->q, kv->sequences, a->q_seq_stride, a->query_heads, a->q_head_stride, kv->head_dim, a->elem};
+  const BufferRows out = {a->out, kv->sequences, a->out_seq_stride, a->query_heads, a->out_head_stride, kv->head_dim, a->elem};
+  if (!rows_distinct(out)) return bad(SI_E_INVALID, "paged attention output rows overlap");
+  if (rows_meet(q, out)) return bad(SI_E_INVALID, "paged attention cannot write its output over the queries");
   if (a->weights_out && a->weights_stride == 0) return bad(SI_E_INVALID, "paged attention weights have no stride");
   if (a->weights_out && uint64_t(kv->sequences) * kv->kv_heads > 65535)
     return bad(SI_E_UNSUPPORTED, "paged attention weights take at most 65535 sequences times kv heads");

@@ -438,3 +438,53 @@ def test_started_arrays_of_an_append(field):
     ctx.device, ctx.h = -1, None
     with pytest.raises(mai.SiError, match="described for a cache"):
         ctx.paged_append_dev(mai.paged_kv(*pools(seqs=5)), made)
+
+
+# ---- buffers that overlap ------------------------------------------------------------
+def elements(at, n0, s0, n1, s1, dims):
+    """Elements of each row of a buffer, by enumeration."""
+    return [set(range(at + i * s0 + j * s1, at + i * s0 + j * s1 + dims)) for i in range(n0) for j in range(n1)]
+
+
+def taken(fn, *args):
+    """Whether the arguments pass; a refusal must name an overlap."""
+    assert fn(None, *[C.byref(a) for a in args], None) == INVALID
+    text = L.si_global_last_error().decode()
+    assert text == "null context" or "over" in text or "apart" in text, text
+    return text == "null context"
+
+
+BASE = 1 << 20  # never read: the calls have no context
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_outputs_over_parts_of_the_inputs_are_refused(seed):
+    """Random places and strides of two buffers against their elements, enumerated: with equal strides the answer
+    is exact, with others a call is taken only if the buffers share nothing."""
+    rng = np.random.default_rng(seed)
+    seen = set()
+    for turn in range(1500):
+        hd, n0, n1 = 8 * int(rng.integers(1, 3)), int(rng.integers(1, 5)), 2 * int(rng.integers(1, 4))
+        strides = sorted((int(rng.choice([hd, hd + 1, hd + 8, 2 * hd, 3 * hd])), int(rng.choice([1, 2, 4, 6, 8]) * (2 * hd + rng.integers(0, 9)))))
+        s1, s0 = strides if rng.random() < 0.7 else strides[::-1]
+        t0, t1 = (s0, s1) if rng.random() < 0.7 else (s0 + 8 * int(rng.integers(0, 3)), s1 + int(rng.integers(0, 2)))
+        at = int(rng.choice([0, 1, hd - 1, hd, 2 * hd, s1, s0, n1 * s1, n0 * s0, int(rng.integers(0, 300))]))
+        swap = rng.random() < 0.5
+        q, out = elements(0, n0, s0, n1, s1, hd), elements(at, n0, t0, n1, t1, hd)
+        alone = sum(map(len, out)) == len(set().union(*out))
+        meet = bool(set().union(*q) & set().union(*out))
+        kv, a = attention_call()
+        kv.sequences, kv.kv_heads, kv.head_dim, a.query_heads, a.work_bytes = n0, n1 // 2, hd, n1, 1 << 40
+        a.q, a.out = (BASE, BASE + 4 * at)
+        a.q_seq_stride, a.q_head_stride, a.out_seq_stride, a.out_head_stride = s0, s1, t0, t1
+        if swap and alone and sum(map(len, q)) == len(set().union(*q)):
+            a.q, a.out = a.out, a.q
+            a.q_seq_stride, a.q_head_stride, a.out_seq_stride, a.out_head_stride = t0, t1, s0, s1
+        ok = taken(L.si_paged_attention_dev, kv, a)
+        same = (n0 == 1 or s0 == t0) and (n1 == 1 or s1 == t1)
+        seen.add((ok, same, alone, meet))
+        assert not ok or (alone and not meet), (turn, hd, n0, n1, s0, s1, t0, t1, at)
+        nested = (s1 >= hd and (n0 == 1 or s0 >= (n1 - 1) * s1 + hd)) or (s0 >= hd and s1 >= (n0 - 1) * s0 + hd)
+        if same and nested and not meet:
+            assert ok, (turn, hd, n0, n1, s0, s1, t0, t1, at)
+    assert {(True, True, True, False), (False, True, True, True), (True, False, True, False), (False, False, True, True)} <= seen
