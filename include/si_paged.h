@@ -105,8 +105,9 @@ int si_rope_table(double theta, uint32_t rotary_dim, const si_rope_scaling* scal
  * they are, rounded to the cache's type, written to slot slot[t] of sequence
  * sequence[t]. A token whose slot is negative is padding: nothing of it is
  * written, neither cache nor q_out. Two tokens of a call must not share a
- * (sequence, slot). q and q_out may be the same memory with the same strides.
- * Strides count elements; dims are contiguous.
+ * (sequence, slot). q and q_out may be the same memory with the same strides;
+ * otherwise no element of q_out is one of q, k or v, nor are its rows each
+ * other's. Strides count elements; dims are contiguous.
  * With weights and positions, the arrays that attention adds to and eviction
  * reads, every appended slot starts with weight 0 and its token's position in
  * each kv head. A slot behind a cut holds what the token that left it had

@@ -255,6 +255,19 @@ int check_append(const si_paged_kv* kv, const si_paged_append* a, std::string* m
                               a->k_token_stride,     a->k_head_stride, a->v_token_stride,     a->v_head_stride};
   for (uint64_t s : strides)
     if (s >> 36) return bad(SI_E_INVALID, "paged append strides are out of range");
+  if (a->tokens && a->q) {
+    const BufferRows q = {a->q, a->tokens, a->q_token_stride, a->query_heads, a->q_head_stride, kv->head_dim, a->elem};
+    const BufferRows out = {a->q_out,          a->tokens,    a->q_out_token_stride, a->query_heads,
+                            a->q_out_head_stride, kv->head_dim, a->elem};
+    if (!rows_distinct(out)) return bad(SI_E_INVALID, "paged append output rows overlap");
+    const bool in_place = q.p == out.p && (q.n0 == 1 || q.s0 == out.s0) && (q.n1 == 1 || q.s1 == out.s1);
+    if (!in_place && rows_meet(q, out))
+      return bad(SI_E_INVALID, "paged append writes its queries in place or apart from those it reads");
+    if (a->k)
+      for (const BufferRows& in : {BufferRows{a->k, a->tokens, a->k_token_stride, kv->kv_heads, a->k_head_stride, kv->head_dim, a->elem},
+                                   BufferRows{a->v, a->tokens, a->v_token_stride, kv->kv_heads, a->v_head_stride, kv->head_dim, a->elem}})
+        if (rows_meet(in, out)) return bad(SI_E_INVALID, "paged append would write queries over new keys or values");
+  }
   return SI_OK;
 }
 

@@ -488,3 +488,32 @@ def test_outputs_over_parts_of_the_inputs_are_refused(seed):
         if same and nested and not meet:
             assert ok, (turn, hd, n0, n1, s0, s1, t0, t1, at)
     assert {(True, True, True, False), (False, True, True, True), (True, False, True, False), (False, False, True, True)} <= seen
+
+
+def test_queries_are_written_in_place_or_apart():
+    """One projection's output [tokens][q, k, v heads]: in place, into free heads, over the keys, shifted by a token."""
+    heads, hd, row = 4, 16, (4 + 2 + 2 + 4) * 16  # queries, keys, values, and as many free heads
+    wide = torch.zeros(3, 12, 16)
+    kv, _ = append_call()
+    n = torch.zeros(3, dtype=torch.int32)
+    q, k, v, free = wide.split([4, 2, 2, 4], 1)
+
+    def call(out):
+        return mai.paged_append(kv, q, k, v, out, n)
+    for out in (q, free, torch.zeros(3, 4, 16)):
+        accepted(L.si_paged_append_dev, kv, call(out))
+    late = torch.as_strided(wide, (3, 4, 16), (row, hd, 1), hd)             # a head further: over the queries and keys
+    over = torch.as_strided(wide, (3, 4, 16), (row, hd, 1), heads * hd)     # over the keys and values
+    turned = torch.as_strided(wide, (3, 4, 16), (hd, 3 * hd, 1), 0)         # the same place in another order
+    flat = torch.zeros(3, 1, 16).expand(3, 4, 16)                           # all heads in one row
+    for out in (late, over, turned, flat):
+        refused(L.si_paged_append_dev, kv, call(out))
+    a = call(free)
+    a.v = a.q_out  # values that the queries would go over
+    refused(L.si_paged_append_dev, kv, a)
+    one = mai.paged_append(kv, q[:1], None, None, q[:1], n[:1])
+    one.q_out_token_stride = 5 * row  # one token has no token stride
+    accepted(L.si_paged_append_dev, kv, one)
+    none = call(late)
+    none.tokens = 0
+    accepted(L.si_paged_append_dev, kv, none)
