@@ -50,7 +50,8 @@ extern "C" {
  * strides. Slot t of sequence b is token t % page_tokens of page
  * pages[b * pages_stride + t / page_tokens]. Entries of the page table that no
  * slot in use needs are not read as pages. Rows of the batch may share pages
- * as long as no operator writes them. */
+ * as long as no operator writes them; pools that are written have every
+ * (page, head, token) in a place of its own. */
 typedef struct si_paged_kv {
   void* k;                  /* pools, 16-byte aligned */
   void* v;

@@ -68,6 +68,10 @@ wide span_of(const BufferRows& r) {
 }  // namespace
 
 bool rows_distinct(const BufferRows& r) { return distinct({{r.n0, r.s0}, {r.n1, r.s1}}, r.dims); }
+bool pools_distinct(const si_paged_kv& kv) {
+  return distinct({{kv.num_pages, kv.page_stride}, {kv.kv_heads, kv.head_stride}, {kv.page_tokens, kv.token_stride}},
+                  kv.head_dim);
+}
 
 bool rows_meet(const BufferRows& a, const BufferRows& b) {
   const wide apart = wide(reinterpret_cast<uintptr_t>(b.p)) - wide(reinterpret_cast<uintptr_t>(a.p));

@@ -178,6 +178,8 @@ struct BufferRows {
 // axes of smaller strides span. (Rows that interleave in no such order count as
 // shared; views of one allocation do not.)
 bool rows_distinct(const BufferRows& r);
+// The same of a cache's pools.
+bool pools_distinct(const si_paged_kv& kv);
 // Whether any element is in both buffers, of one element type. Exact where the
 // strides are the same (parts of one buffer); otherwise buffers whose ranges
 // overlap count as sharing.

@@ -268,6 +268,8 @@ int check_append(const si_paged_kv* kv, const si_paged_append* a, std::string* m
                                    BufferRows{a->v, a->tokens, a->v_token_stride, kv->kv_heads, a->v_head_stride, kv->head_dim, a->elem}})
         if (rows_meet(in, out)) return bad(SI_E_INVALID, "paged append would write queries over new keys or values");
   }
+  if (a->tokens && a->k && (!pools_distinct(*kv) || kv->k == kv->v))
+    return bad(SI_E_INVALID, "paged append needs pools whose rows do not overlap");
   return SI_OK;
 }
 

@@ -426,6 +426,7 @@ int check_evict(const si_paged_kv* kv, const si_paged_evict* a, std::string* msg
   };
   if (!a) return bad(SI_E_INVALID, "null paged eviction description");
   if (int rc = check_size(kv, msg)) return rc;
+  if (!pools_distinct(*kv)) return bad(SI_E_INVALID, "paged eviction needs pools whose rows do not overlap");
   if (!a->lengths_in || !a->lengths_out || !a->weights_in || !a->weights_out)
     return bad(SI_E_INVALID, "paged eviction buffers are null");
   if (!words_aligned({a->lengths_in, a->lengths_out, a->weights_in, a->weights_out, a->positions_in, a->positions_out,

@@ -517,3 +517,25 @@ def test_queries_are_written_in_place_or_apart():
     none = call(late)
     none.tokens = 0
     accepted(L.si_paged_append_dev, kv, none)
+
+
+@pytest.mark.parametrize("name", ["append", "evict"])
+def test_pools_with_shared_rows_are_not_written(name):
+    """Pools expanded over heads or pages can be attended and not written."""
+    make, fn = CALLS[name]
+    flat = torch.zeros(7, 1, 4, 16, dtype=torch.bfloat16)[:6]
+    for k in (flat.expand(6, 2, 4, 16), flat[:1].expand(6, 1, 4, 16), torch.as_strided(flat, (6, 2, 4, 16), (64, 8, 16, 1))):
+        v = torch.as_strided(torch.zeros(7, 1, 4, 16, dtype=torch.bfloat16), k.shape, k.stride())
+        refused(fn, mai.paged_kv(k, v, torch.zeros(3, 2, dtype=torch.int32)), make()[1])
+        assert "overlap" in L.si_global_last_error().decode()
+    kv, a = make()
+    kv.num_pages, kv.page_stride = 1, 0  # one page has no stride
+    accepted(fn, kv, a)
+    q = torch.zeros(3, 4, 16)
+    shared = mai.paged_kv(flat.expand(6, 2, 4, 16), flat.expand(6, 2, 4, 16), torch.zeros(3, 2, dtype=torch.int32))
+    work = torch.zeros(mai.paged_attention_workspace_bytes(shared, 4) // 8 + 2, dtype=torch.float64)
+    accepted(L.si_paged_attention_dev, shared, mai.paged_attention(shared, q, torch.zeros_like(q), torch.zeros(3, dtype=torch.int32), work))
+    if name == "append":
+        kv, a = make()
+        kv.v = kv.k
+        refused(fn, kv, a)
