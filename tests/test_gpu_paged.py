@@ -1170,3 +1170,81 @@ def test_append_leaves_out_the_queries_of_bad_tokens(ctx):
     with pytest.raises(mai.SiError):
         ctx.synchronize()
     assert torch.equal(out[[0, 4]], q[[0, 4]]) and (out[1:4] == 7).all()
+
+
+def evicted_rows(w, pos, n, budget, sink, recent, nxt):
+    """`evicted` by numpy: (holes, kept slots behind the budget) of one row of finite weights."""
+    held = (pos[:n] < sink) | (pos[:n] >= nxt - recent)
+    order = np.lexsort((np.arange(n), np.where(held, 0, w[:n]), held))  # protected last, by weight, by slot
+    gone = np.zeros(n, bool)
+    gone[order[:max(0, n - budget)]] = True
+    m = min(n, budget)
+    return np.flatnonzero(gone[:m]), m + np.flatnonzero(~gone[m:])
+
+
+EVICT_MANY = [
+    # sequences, kv_heads, longest, budget: rows that outnumber the clusters' places, and the largest row
+    (64, 1, 8193, 8100),     # 1024 threads, no cluster, moves in the same kernel (not over its own lengths)
+    (19, 3, 20000, 9000),    # the same, moves in a second kernel
+    (57, 1, 49152, 49100),   # the most keys of one CTA
+    (5, 2, 70000, 4000),     # clusters of 8 cut to 6
+    (10, 2, 60000, 30000),   # to 4
+    (15, 2, 90000, 89990),   # to 2, 45,000 keys a CTA
+    (1, 1, 393216, 200000),  # the longest row, the most keys in each CTA of a cluster of 8
+    (1, 1, 393216, 393215),
+]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("case", range(len(EVICT_MANY)))
+def test_evict_many_and_long_rows(ctx, case, in_place):
+    seqs, kvh, longest, budget = EVICT_MANY[case]
+    rng = np.random.default_rng(case)
+    lengths = [longest] + [int(x) for x in rng.integers(budget // 2, longest + 1, seqs - 1)]
+    if seqs > 4:
+        lengths[3], lengths[-1] = 0, longest
+    hd, sink, recent, page = 8, 3, 40, 4096
+    cache = Cache(lengths, kvh, page, hd, BF16, seed=case, cols=-(-longest // page))
+    cache.k.nan_to_num_(0.0), cache.v.nan_to_num_(0.0)
+    shape = (seqs, kvh, longest)
+    w = (np.floor(np.exp(2 * rng.normal(size=shape)) * 64) / 64).astype(np.float32)  # many ties among the small ones
+    pos = np.broadcast_to(np.arange(longest, dtype=np.int32), shape).copy()
+    w_in, p_in = torch.from_numpy(w).cuda(), torch.from_numpy(pos).cuda()
+    w_out = w_in if in_place else torch.full_like(w_in, 3.5)
+    p_out = p_in if in_place else torch.full_like(p_in, -9)
+    n_out = cache.len_dev if in_place else torch.full_like(cache.len_dev, -1)
+    work = torch.empty(mai.paged_evict_workspace_bytes(cache.desc), dtype=torch.uint8, device="cuda").fill_(255)
+    k0, v0 = cache.k.clone(), cache.v.clone()
+    ctx.paged_evict_dev(cache.desc, mai.paged_evict(cache.desc, cache.len_dev, n_out, w_in, w_out, budget, work, sink=sink, recent=recent,
+                                                    positions_in=p_in, positions_out=p_out), LEGACY)
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    assert n_out.tolist() == [min(n, budget) for n in lengths]
+    want_w = w.copy() if in_place else np.full_like(w, 3.5)
+    want_p = pos.copy() if in_place else np.full_like(pos, -9)
+    for b, n in enumerate(lengths):
+        m = min(n, budget)
+        pg, at = cache.cells(b, n)
+        for h in range(kvh):
+            holes, movers = evicted_rows(w[b, h], pos[b, h], n, budget, sink, recent, n)
+            assert len(holes) == len(movers)
+            want_w[b, h, :m], want_p[b, h, :m] = w[b, h, :m], pos[b, h, :m]
+            want_w[b, h, holes], want_p[b, h, holes] = w[b, h, movers], pos[b, h, movers]
+            to, of = torch.from_numpy(holes).cuda(), torch.from_numpy(movers).cuda()
+            for pool, start in ((cache.k, k0), (cache.v, v0)):
+                moved = start[pg[of], h, at[of]].clone()
+                assert torch.equal(pool[pg[to], h, at[to]], moved)
+                pool[pg[to], h, at[to]] = start[pg[to], h, at[to]]
+    np.testing.assert_array_equal(w_out.cpu().numpy().view(np.uint32), want_w.view(np.uint32))
+    np.testing.assert_array_equal(p_out.cpu().numpy(), want_p)
+    assert torch.equal(cache.k, k0) and torch.equal(cache.v, v0)
+
+
+def test_evicted_rows_agree_with_the_definition():
+    rng = np.random.default_rng(1)
+    for n in (1, 7, 60):
+        for budget in (1, 5, 30, 60):
+            w = np.floor(rng.random(n) * 4).astype(np.float32)
+            pos = rng.permutation(2 * n)[:n].astype(np.int32)
+            holes, movers = evicted_rows(w, pos, n, budget, 1, min(3, budget - 1), 2 * n)
+            assert (holes.tolist(), movers.tolist()) == evicted(w, pos, n, budget, 1, min(3, budget - 1), 2 * n)
