@@ -1248,3 +1248,120 @@ def test_evicted_rows_agree_with_the_definition():
             pos = rng.permutation(2 * n)[:n].astype(np.int32)
             holes, movers = evicted_rows(w, pos, n, budget, 1, min(3, budget - 1), 2 * n)
             assert (holes.tolist(), movers.tolist()) == evicted(w, pos, n, budget, 1, min(3, budget - 1), 2 * n)
+
+
+def test_two_contexts_in_two_threads(ctx):
+    """Two host threads with contexts of their own launch the same kernels with different sizes, and so different
+    shared-memory needs, at once."""
+    import threading
+    failures = []
+
+    def work(lengths, rows, seed):
+        try:
+            own, stream = mai.CudaContext(0), torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                cache = Cache(lengths, 1, 16, 64, BF16, seed=seed)
+                q = torch.randn(len(lengths), 2, 64, device="cuda")
+                out, scratch = torch.empty_like(q), work_for(cache, 2)
+                attention = mai.paged_attention(cache.desc, q, out, cache.len_dev, scratch)
+                long = Cache([rows], 1, 256, 8, F16, seed=seed)
+                w, n_out = torch.rand(1, 1, rows, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+                w_out = torch.empty_like(w)
+                evict = mai.paged_evict(long.desc, long.len_dev, n_out, w, w_out, rows - 1,
+                                        torch.empty(mai.paged_evict_workspace_bytes(long.desc), dtype=torch.uint8, device="cuda"))
+                for _ in range(30):
+                    own.paged_attention_dev(cache.desc, attention, stream.cuda_stream)
+                    own.paged_evict_dev(long.desc, evict, stream.cuda_stream)
+                stream.synchronize()
+                own.synchronize()
+                close(out, reference(cache, q)[0], F32)
+                assert n_out.item() == rows - 1
+                least = w[0, 0].argmin().item()
+                assert least >= rows - 1 or w_out[0, 0, least] == w[0, 0, rows - 1]
+            own.close()
+        except BaseException as e:  # noqa: BLE001 - reported by the test's own thread
+            failures.append(e)
+    threads = [threading.Thread(target=work, args=x) for x in (([5, 900], 1900, 1), ([3] * 4000, 1000, 2), ([17] * 700, 2040, 3))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not failures and not any(t.is_alive() for t in threads), failures
+
+
+def test_a_captured_step_with_forks_and_copies(ctx):
+    """One graph: inputs copied in, the append, then attention and verification on two branches that meet again,
+    the eviction, a copy out. Replayed with other inputs."""
+    kvh, g, hd, vocab = 2, 2, 64, 501
+    cache = Cache([40, 17], kvh, 8, hd, BF16, seed=21, room=1)
+    start_k, start_v = cache.k.clone(), cache.v.clone()
+    host_q = torch.randn(2, kvh * g, hd, device="cuda")
+    q, out = torch.empty_like(host_q), torch.empty_like(host_q)
+    k = torch.randn(2, kvh, hd, device="cuda").to(BF16)
+    length0 = torch.tensor([40, 17], dtype=torch.int32, device="cuda")
+    slot, length = length0.clone(), length0 + 1
+    weights, positions = torch.zeros(2, kvh, 48, device="cuda"), torch.zeros(2, kvh, 48, dtype=torch.int32, device="cuda")
+    w_out, n_out = torch.empty_like(weights), torch.empty_like(length)
+    p = torch.rand(2, 2, vocab, device="cuda")
+    tokens, u, last = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.rand(2, 1, device="cuda"), torch.rand(2, device="cuda")
+    accepted, following, copied = (torch.empty(2, dtype=torch.int32, device="cuda") for _ in range(3))
+    append = mai.paged_append(cache.desc, None, k, k, None, slot, weights=weights, positions=positions)
+    attention = mai.paged_attention(cache.desc, q, out, length, work_for(cache, kvh * g, True), weights_in=weights, weights_out=weights)
+    verify = mai.verify_drafts(p, tokens, u, last, accepted, following, torch.empty(16, dtype=torch.uint8, device="cuda"))
+    evict = mai.paged_evict(cache.desc, length, n_out, weights, w_out, 30,
+                            torch.empty(mai.paged_evict_workspace_bytes(cache.desc), dtype=torch.uint8, device="cuda"))
+    main, side, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=main):
+        q.copy_(host_q)
+        ctx.paged_append_dev(cache.desc, append, main.cuda_stream)
+        side.wait_stream(main)
+        ctx.verify_drafts_dev(verify, side.cuda_stream)
+        ctx.paged_attention_dev(cache.desc, attention, main.cuda_stream)
+        main.wait_stream(side)
+        ctx.paged_evict_dev(cache.desc, evict, main.cuda_stream)
+        copied.copy_(n_out)
+    for turn in range(3):
+        host_q.normal_(), k.normal_(), u.uniform_(), last.uniform_(), p.uniform_()
+        cache.k.copy_(start_k), cache.v.copy_(start_v)
+        weights.uniform_(), positions.fill_(-1)
+        before = weights.clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        ctx.synchronize()
+        assert copied.tolist() == [30, 18]
+        for b, n in enumerate((41, 18)):
+            keys = torch.cat([start_k[cache.cells(b, n - 1)[0], :, cache.cells(b, n - 1)[1]], k[b:b + 1]]).double()
+            values = torch.cat([start_v[cache.cells(b, n - 1)[0], :, cache.cells(b, n - 1)[1]], k[b:b + 1]]).double()
+            prob = torch.softmax(torch.einsum("hgd,nhd->hgn", host_q[b].double().view(kvh, g, hd), keys) / 8, -1)
+            close(out[b], torch.einsum("hgn,nhd->hgd", prob, values).reshape(kvh * g, hd), F32)
+            before[b, :, n - 1] = 0
+            close(weights[b, :, :n], before[b, :, :n].double() + prob.sum(1), F32)
+            assert (positions[b, :, n - 1] == n - 1).all() and (positions[b, :, :n - 1] == -1).all()
+            for h in range(kvh):
+                holes, movers = evicted(weights[b, h].tolist(), list(range(48)), n, 30, 0, 0, n)
+                got = weights[b, h, :min(n, 30)].clone()
+                got[holes] = weights[b, h, movers]
+                assert torch.equal(w_out[b, h, :min(n, 30)], got)
+            assert (accepted[b].item(), following[b].item()) == verified(p[b].cpu().numpy(), None, tokens[b].tolist(), u[b].tolist(),
+                                                                         last[b].item(), 1)
+
+
+def test_evict_with_one_array_of_lengths(ctx):
+    """Lengths in, lengths out and next positions in one array: the last `recent` slots of each row are protected."""
+    cache = Cache([50, 12, 33], 2, 8, 64, BF16, seed=9)
+    n = cache.len_dev.clone()
+    w = torch.rand(3, 2, 64, device="cuda")
+    w[:, :, 25:] = 0  # the last ones would leave first
+    before = w.clone()
+    work = torch.empty(mai.paged_evict_workspace_bytes(cache.desc), dtype=torch.uint8, device="cuda")
+    ctx.paged_evict_dev(cache.desc, mai.paged_evict(cache.desc, n, n, w, w, 20, work, recent=10, next_position=n), LEGACY)
+    assert n.tolist() == [20, 12, 20]
+    for b, m in enumerate((50, 12, 33)):
+        for h in range(2):
+            holes, movers = evicted(before[b, h].tolist(), list(range(64)), m, 20, 0, 10, m)
+            want = before[b, h].clone()
+            want[holes] = before[b, h, movers]
+            assert torch.equal(w[b, h, :min(m, 20)], want[:min(m, 20)])
+    ctx.synchronize()
