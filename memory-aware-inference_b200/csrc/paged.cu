@@ -48,16 +48,16 @@ using wide = __int128;
 struct Axis {
   uint64_t n, stride;
 };
-bool distinct(std::initializer_list<Axis> given, uint32_t dims) {
-  Axis axes[3];
-  int count = 0;
-  for (const Axis& a : given)
-    if (a.n > 1) axes[count++] = a;
-  std::sort(axes, axes + count, [](const Axis& a, const Axis& b) { return a.stride < b.stride; });
+// Axes sorted by hand: three at most, and a call is bound by its host time.
+bool distinct(Axis a, Axis b, Axis c, uint32_t dims) {
+  if (a.stride > b.stride) std::swap(a, b);
+  if (b.stride > c.stride) std::swap(b, c);
+  if (a.stride > b.stride) std::swap(a, b);
   wide span = dims;
-  for (int i = 0; i < count; ++i) {
-    if (wide(axes[i].stride) < span) return false;
-    span += wide(axes[i].n - 1) * axes[i].stride;
+  for (const Axis& x : {a, b, c}) {
+    if (x.n <= 1) continue;
+    if (wide(x.stride) < span) return false;
+    span += wide(x.n - 1) * x.stride;
   }
   return true;
 }
@@ -67,9 +67,9 @@ wide span_of(const BufferRows& r) {
 }
 }  // namespace
 
-bool rows_distinct(const BufferRows& r) { return distinct({{r.n0, r.s0}, {r.n1, r.s1}}, r.dims); }
+bool rows_distinct(const BufferRows& r) { return distinct({r.n0, r.s0}, {r.n1, r.s1}, {1, 0}, r.dims); }
 bool pools_distinct(const si_paged_kv& kv) {
-  return distinct({{kv.num_pages, kv.page_stride}, {kv.kv_heads, kv.head_stride}, {kv.page_tokens, kv.token_stride}},
+  return distinct({kv.num_pages, kv.page_stride}, {kv.kv_heads, kv.head_stride}, {kv.page_tokens, kv.token_stride},
                   kv.head_dim);
 }
 
