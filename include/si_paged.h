@@ -99,7 +99,8 @@ typedef struct si_rope_scaling {
 /* Host only: the frequencies as turns (2 pi radians) a position in units of
  * 2^-64, [rotary_dim / 2], and the factor on rotated values. `scaling` NULL:
  * NONE. position * turn in 64-bit integers is the pair's angle modulo one
- * turn, exact at any position. The caller copies the table to the device. */
+ * turn, off by the table's own rounding only: at most |position| * 2^-65
+ * turns. The caller copies the table to the device. */
 int si_rope_table(double theta, uint32_t rotary_dim, const si_rope_scaling* scaling, uint64_t* turns, float* scale);
 
 /* For every token t: queries rotated into q_out; keys rotated and values as
@@ -140,13 +141,16 @@ int si_paged_append_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_appen
  * own key and value are in the cache already (si_paged_append_dev). A sequence
  * of length 0 gets zeros (and lse = -inf): rows of a padded batch have length
  * 0. Cached values at slots in use are taken to be finite; whatever lies in
- * other slots is not read. Sums and the softmax are held in f32, with f32
- * queries and f32 output the products too. The same call gives the same bits;
- * how the sums group depends on all lengths of the batch.
+ * other slots is not read. Sums and the softmax are held in f32. With f32
+ * queries and output the products keep 24 bits of queries and probabilities
+ * over a bf16 cache and 22 bits over an f16 cache; with queries of the cache's
+ * own 16-bit type, probabilities keep 16 bits (bf16) or 22 (f16). The same
+ * call gives the same bits; how the sums group depends on all lengths of the
+ * batch.
  * With weights_out, weights_out[b][h][t] = weights_in[b][h][t] + the sum of
  * the probabilities of slot t over the query heads of kv head h, for
  * t < lengths[b]; other entries are left as they are. weights_in may be
- * weights_out, or NULL for zeros. */
+ * weights_out (otherwise they share nothing), or NULL for zeros. */
 typedef struct si_paged_attention {
   const void* q;            /* [sequences][query_heads][head_dim] */
   void* out;                /* no element of q: several blocks read a query; rows apart from each other */
@@ -162,7 +166,12 @@ typedef struct si_paged_attention {
   void* work;               /* 16-byte aligned */
   uint64_t work_bytes;
 } si_paged_attention;
-/* Host only: bytes of workspace a call needs (with or without weights). */
+/* Host only: bytes of workspace a call needs (with or without weights). With
+ * weights every score is kept between two kernels: sequences * kv_heads *
+ * max_pages * page_tokens * (group of query heads, rounded up to even) * 4
+ * bytes, by the room of the page table, not by the lengths or the pool. 64
+ * sequences with tables for 131,072 slots, 8 kv heads and groups of 4 need
+ * 1.07 GB. */
 int si_paged_attention_workspace(const si_paged_kv* kv, uint32_t query_heads, int weights, uint64_t* bytes);
 int si_paged_attention_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_attention* a, void* stream);
 
@@ -181,7 +190,10 @@ int si_paged_attention_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_at
  * Should more than `budget` tokens be protected (positions that repeat),
  * the protected ones of the lowest slots leave, after all others.
  * Entries of weights_out and positions_out at slots below the new length are
- * written, others left as they are. Each `_in` may be its `_out`. */
+ * written, others left as they are. Each `_in` may be its `_out`; otherwise
+ * inputs and outputs share nothing. Launches are planned for the most slots
+ * that the page table and weights_stride have room for (lengths are on the
+ * device): tables much wider than the rows cost time. */
 typedef struct si_paged_evict {
   const int32_t* lengths_in;    /* [sequences] */
   int32_t* lengths_out;         /* min(length, budget) */
@@ -206,8 +218,10 @@ int si_paged_evict_dev(si_ctx* ctx, const si_paged_kv* kv, const si_paged_evict*
  * accepted ones is drawn from max(target - draft, 0) of the first rejected
  * place, or from the target's row after the last draft when all are accepted:
  * the lowest token whose cumulative weight exceeds last_uniform[b] times the
- * total. Products and sums are held in 64 bits, so the result does not depend
- * on how the work is split. Negative, infinite and NaN entries count as 0. If
+ * total. Acceptance is exact, and sums are held in 64 bits. The same call gives
+ * the same token; in a batch of another size a row's sums are taken in another
+ * order, which moves a border by about 1e-16 of the total and so the token
+ * about once in 10^10 draws. Negative, infinite and NaN entries count as 0. If
  * the difference is 0 everywhere the target's row itself is drawn from; if that
  * is too, next = -1. draft NULL: the drafter has no probabilities (1 for its
  * token): x is accepted with probability target[x], and the difference is the
@@ -222,14 +236,14 @@ typedef struct si_verify_drafts {
   const float* uniform;     /* [sequences][drafts] in [0, 1) */
   const float* last_uniform;/* [sequences] in [0, 1) */
   int32_t* accepted;        /* [sequences]; may be counts */
-  int32_t* next;            /* [sequences] */
+  int32_t* next;            /* [sequences]; not accepted */
   uint32_t sequences;       /* at most 65535 */
   uint32_t drafts;          /* 0..32 */
   uint32_t vocab;           /* below 2^31 */
   void* work;               /* 16-byte aligned */
   uint64_t work_bytes;
 } si_verify_drafts;
-/* Host only. */
+/* Host only. 16 bytes for any call; the operator keeps nothing in them. */
 int si_verify_drafts_workspace(uint32_t sequences, uint32_t vocab, uint64_t* bytes);
 int si_verify_drafts_dev(si_ctx* ctx, const si_verify_drafts* a, void* stream);
 

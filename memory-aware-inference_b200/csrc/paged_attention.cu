@@ -1,9 +1,10 @@
 // Attention of one new token a sequence over a paged key-value cache.
 //
 // o = sum_t p_t v_t / sum_t p_t, p_t = exp(s_t - max s), s_t = scale q.k_t, for
-// the query heads that share a kv head. Every key and value is read once, so
-// the work is bound by HBM (2 flop a byte and query head) once a few thousand
-// tokens are in the batch, and by latency below that.
+// the query heads that share a kv head. Up to 8 query heads a kv head read every
+// key and value once, so the work is bound by HBM (2 flop a byte and query head)
+// once a few thousand tokens are in the batch, and by latency below that. Larger
+// groups are several blocks of 8 heads, each of which reads all of them.
 //
 // Split. The unit of work is 16 consecutive slots of one (sequence, kv head,
 // block of 8 query heads), a pair. All units of the batch, in that order, are
@@ -16,8 +17,9 @@
 // CTA) in the workspace, which a second kernel joins. Every join sums in a fixed order.
 // A worker is a warp; for head_dim above 192 two warps, each with half of the
 // dims, that exchange their halves of the scores once a unit (one call of 517
-// slots of 256 dims 13.6 us where one warp a unit takes 14.8, 65,536 slots with bf16
-// queries 53 and 56, 131,071 with f32 ones 110 and 107).
+// slots of 256 dims 13.0 us where one warp a unit takes 14.5, 65,536 slots with bf16
+// queries 53 and 56; long rows with f32 queries are 2 % slower, 131,071 slots
+// 115.6 and 113, 8 rows of 8,192 with weights 62.7 and 61.3).
 //
 // A unit. Keys and values go from global memory straight into the registers
 // in which the tensor cores (mma.m16n8k16) want them; there is no shared-memory
@@ -36,15 +38,16 @@
 // The keys of the next unit are requested when this unit's scores are done,
 // its values step by step as this unit's are used, so loads are in flight
 // throughout. What bounds it: HBM for 16-bit queries (64 ragged sequences, 0.69 GB
-// in 115 us, 6.0 TB/s), the latency of a unit for f32 ones (0.54 GB in 114 us).
+// in 116 us, 6.0 TB/s), the latency of a unit for f32 ones (0.54 GB in 113 us).
 //
 // Precision: queries are split into TQ 16-bit terms and probabilities into TP,
-// each multiplied separately into the same f32 accumulators. 16-bit queries of
-// the cache's own type are exact in one term. f32 queries take 3 bf16 terms
-// (24 bits) or 2 f16 terms (22 bits, after scaling each query by a power of two
-// to a maximum near 2^15), probabilities 3 bf16 or 2 f16 terms with f32 output and
-// 2 with 16-bit output. In f16, probabilities are scaled up so that small ones keep their
-// bits; the sum is taken of the same scaled values.
+// each multiplied separately into f32 sums. 16-bit queries of the cache's own
+// type are exact in one term, and probabilities then take 2 (16 bits in bf16, 22
+// in f16: the output keeps 8 or 11). All other queries (f32, or the other 16-bit
+// type) take 3 bf16 terms (24 bits) or 2 f16 terms (22 bits, after scaling each
+// query by a power of two to a maximum near 2^15), and probabilities as many. In
+// f16, probabilities are scaled up so that small ones keep their bits; the sum is
+// taken of the same scaled values.
 #include <cuda_runtime.h>
 
 #include <algorithm>

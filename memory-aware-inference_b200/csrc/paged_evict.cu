@@ -16,7 +16,7 @@
 // chain of small scans, so as many rows as possible run beside each other.
 // Moves: a second kernel over all pairs of all heads, because a cut of a long
 // prompt moves megabytes where the selection is a few scans. Selection is bound by
-// latency, moves by bandwidth: 16 rows of 131,072 slots cut to 8,192 take 78 us, of
+// latency, moves by bandwidth: 16 rows of 131,072 slots cut to 8,192 take 77 us, of
 // which the moves are 42 (252 MB, 6 TB/s).
 #include <cuda_runtime.h>
 
@@ -483,7 +483,7 @@ extern "C" int si_paged_evict_dev(si_ctx* ctx, const si_paged_kv* kv, const si_p
   // graphics processing cluster has 14 multiprocessors or more, so 8 of them hold
   // 8 (14 / c) clusters of c CTAs for sure. Multiprocessors come in pairs, and odd
   // sizes were slower than the even ones on both sides (16 rows of 131,072 slots:
-  // clusters of 8, in two waves, 110 us; 7, 98; 6, 82; 5, 84; 4, 88).
+  // clusters of 8, in two waves, 92 us; 7, 95; 6, 77; 5, 78; 4, 86).
   uint32_t cluster = std::min(kMaxCluster, (most + 8191) / 8192);
   if (cluster > 1) cluster += cluster % 2;
   while (cluster > 1 && rows > 8 * (14 / cluster) && most <= (cluster > 2 ? cluster - 2 : 1) * kCtaSlots)
@@ -491,7 +491,7 @@ extern "C" int si_paged_evict_dev(si_ctx* ctx, const si_paged_kv* kv, const si_p
   const uint32_t each = (most + cluster - 1) / cluster;
   // Moves of one row are at most the smaller of both sides of the budget. A few
   // (a page's worth leaves in steady state) the selecting CTA makes itself, which saves a
-  // launch: 32 x 8 rows of 4,160 slots that lose 64 take 16.9 us, and 19.5 us with a second
+  // launch: 32 x 8 rows of 4,160 slots that lose 64 take 16.0 us, and 18.6 us with a second
   // kernel. Not where the new lengths go over the old ones: other heads' CTAs
   // still read those.
   const uint64_t most_moves = std::min<uint64_t>(most > a->budget ? most - a->budget : 0, a->budget);

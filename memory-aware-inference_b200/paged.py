@@ -153,7 +153,6 @@ def paged_kv(k, v, pages) -> SiPagedKv:
     kv = SiPagedKv(k.data_ptr(), v.data_ptr(), pages.data_ptr(), k.shape[0], k.stride(0), k.stride(1), k.stride(2),
                    max(pages.stride(0), pages.shape[1]) if pages.shape[0] == 1 else pages.stride(0),
                    _elem(k), k.shape[1], k.shape[3], k.shape[2], pages.shape[0], pages.shape[1])
-    kv.device = k.device
     return kv._hold(k, v, pages)
 
 
