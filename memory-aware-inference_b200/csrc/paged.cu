@@ -42,29 +42,27 @@ int check_paged_kv(const si_paged_kv* kv, std::string* msg) {
   return SI_OK;
 }
 
+// Overlaps, in elements. Checked descriptions keep every span below 2^61, so
+// 64-bit sums of three of them do not overflow. Calls are bound by their host
+// time, so what is usual is found out in a few operations.
 namespace {
-using wide = __int128;
-
 struct Axis {
   uint64_t n, stride;
 };
-// Axes sorted by hand: three at most, and a call is bound by its host time.
 bool distinct(Axis a, Axis b, Axis c, uint32_t dims) {
   if (a.stride > b.stride) std::swap(a, b);
   if (b.stride > c.stride) std::swap(b, c);
   if (a.stride > b.stride) std::swap(a, b);
-  wide span = dims;
+  uint64_t span = dims;
   for (const Axis& x : {a, b, c}) {
     if (x.n <= 1) continue;
-    if (wide(x.stride) < span) return false;
-    span += wide(x.n - 1) * x.stride;
+    if (x.stride < span) return false;
+    span += (x.n - 1) * x.stride;
   }
   return true;
 }
-// Bytes from the first element to behind the last.
-wide span_of(const BufferRows& r) {
-  return (wide(r.n0 - 1) * r.s0 + wide(r.n1 - 1) * r.s1 + r.dims) * elem_bytes(r.elem);
-}
+// From the first element to behind the last.
+int64_t span_of(const BufferRows& r) { return int64_t((r.n0 - 1) * r.s0 + (r.n1 - 1) * r.s1 + r.dims); }
 }  // namespace
 
 bool rows_distinct(const BufferRows& r) { return distinct({r.n0, r.s0}, {r.n1, r.s1}, {1, 0}, r.dims); }
@@ -74,24 +72,30 @@ bool pools_distinct(const si_paged_kv& kv) {
 }
 
 bool rows_meet(const BufferRows& a, const BufferRows& b) {
-  const wide apart = wide(reinterpret_cast<uintptr_t>(b.p)) - wide(reinterpret_cast<uintptr_t>(a.p));
+  // both are aligned to their elements
+  const int64_t apart = (static_cast<const char*>(b.p) - static_cast<const char*>(a.p)) / int64_t(elem_bytes(a.elem));
   if (apart >= span_of(a) || -apart >= span_of(b)) return false;
   // an axis of one row has no stride of its own
   if ((a.n0 > 1 && b.n0 > 1 && a.s0 != b.s0) || (a.n1 > 1 && b.n1 > 1 && a.s1 != b.s1)) return true;
-  const wide s0 = a.n0 > 1 ? a.s0 : b.s0, s1 = a.n1 > 1 ? a.s1 : b.s1, elem = elem_bytes(a.elem);
+  const int64_t s0 = int64_t(a.n0 > 1 ? a.s0 : b.s0), s1 = int64_t(a.n1 > 1 ? a.s1 : b.s1), dims = a.dims;
+  // Parts of one buffer mostly: every step of one axis holds all of a's other axis, then all of b's.
+  auto beside = [&](int64_t outer, int64_t inner, uint64_t in_a, uint64_t in_b) {
+    if (outer == 0) return false;
+    const int64_t at = (apart % outer + outer) % outer;
+    return at >= int64_t(in_a - 1) * inner + dims && at + int64_t(in_b - 1) * inner + dims <= outer;
+  };
+  if (beside(s0, s1, a.n1, b.n1) || beside(s1, s0, a.n0, b.n0)) return false;
   // Rows (i0, i1) of a and (j0, j1) of b share an element if |apart - (i0 - j0) s0 -
-  // (i1 - j1) s1| < dims. The shorter axis is walked, the nearest step of the other computed.
+  // (i1 - j1) s1| < dims. The shorter axis is walked, the nearest steps of the other computed.
   struct Steps {
-    wide lo, hi, stride;
-  } x = {-wide(b.n0 - 1), wide(a.n0 - 1), s0}, y = {-wide(b.n1 - 1), wide(a.n1 - 1), s1};
+    int64_t lo, hi, stride;
+  } x = {1 - int64_t(b.n0), int64_t(a.n0) - 1, s0}, y = {1 - int64_t(b.n1), int64_t(a.n1) - 1, s1};
   if (x.hi - x.lo < y.hi - y.lo) std::swap(x, y);
-  const wide dims = wide(a.dims) * elem;
-  for (wide i = y.lo; i <= y.hi; ++i) {
-    const wide rest = apart - i * y.stride * elem;
-    wide near = x.stride ? rest / (x.stride * elem) : 0;
-    for (wide k : {near - 1, near, near + 1}) {
-      k = std::min(std::max(k, x.lo), x.hi);
-      const wide left = rest - k * x.stride * elem;
+  for (int64_t i = y.lo; i <= y.hi; ++i) {
+    const int64_t rest = apart - i * y.stride;
+    const int64_t near = std::min(std::max(x.stride ? rest / x.stride : 0, x.lo), x.hi);
+    for (int64_t k = std::max(near - 1, x.lo); k <= std::min(near + 1, x.hi); ++k) {
+      const int64_t left = rest - k * x.stride;
       if (left > -dims && left < dims) return true;
     }
   }

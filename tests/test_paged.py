@@ -539,3 +539,34 @@ def test_pools_with_shared_rows_are_not_written(name):
         kv, a = make()
         kv.v = kv.k
         refused(fn, kv, a)
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_queries_over_keys_of_any_strides(seed):
+    """Random keys (heads and tokens that may share rows: inputs may be expanded) beside the rotated queries, against
+    their elements: a call is taken only if they share nothing, and always if their strides agree and they do not."""
+    rng = np.random.default_rng(seed)
+    seen = set()
+    for turn in range(1500):
+        hd, tokens, qh, kvh = 8 * int(rng.integers(1, 3)), int(rng.integers(1, 5)), int(rng.integers(1, 5)), int(rng.integers(1, 4))
+        s1 = int(rng.choice([hd, hd + 8, 2 * hd]))
+        s0 = int(rng.choice([1, 2])) * (qh + kvh) * s1 + int(rng.integers(0, 2)) * 8
+        if rng.random() < 0.3:  # tokens inside, heads outside
+            s0, s1 = s1, s0 * tokens
+        t0, t1 = (s0, s1) if rng.random() < 0.6 else (int(rng.choice([0, 1, 8, s0])), int(rng.choice([0, 1, 8, s1])))
+        at = int(rng.choice([0, hd, qh * s1, kvh * s1, s0, tokens * s0, int(rng.integers(0, 400))])) * int(rng.choice([1, -1]))
+        out, k = elements(0, tokens, s0, qh, s1, hd), elements(at, tokens, t0, kvh, t1, hd)
+        meet = bool(set().union(*k) & set().union(*out))
+        kv, a = append_call()
+        kv.kv_heads, kv.head_dim, kv.page_stride, kv.head_stride, kv.token_stride = kvh, hd, 4 * kvh * hd, 4 * hd, hd
+        a.tokens, a.query_heads, a.rotary_dim, a.sequence = tokens, qh, 0, BASE
+        a.q, a.q_out, a.k, a.v = 2 * BASE, 64 * BASE, 64 * BASE + 4 * at, BASE
+        a.q_token_stride, a.q_head_stride, a.q_out_token_stride, a.q_out_head_stride = qh * hd, hd, s0, s1
+        a.k_token_stride, a.k_head_stride, a.v_token_stride, a.v_head_stride = t0, t1, kvh * hd, hd
+        ok = taken(L.si_paged_append_dev, kv, a)
+        same = (tokens == 1 or t0 == s0) and (qh == 1 or kvh == 1 or t1 == s1)
+        seen.add((ok, same, meet))
+        assert not (ok and meet), (turn, hd, tokens, qh, kvh, s0, s1, t0, t1, at)
+        if same and not meet:
+            assert ok, (turn, hd, tokens, qh, kvh, s0, s1, t0, t1, at)
+    assert {(True, True, False), (False, True, True), (True, False, False), (False, False, True)} <= seen
